@@ -142,6 +142,16 @@ int ixb_softmax_layernorm(int dtype, const void* x, const void* g, const void* g
 int ixb_rmsnorm(int dtype, const void* x, const void* res, const void* w, void* y, void* h_out,
                 int64_t rows, int64_t cols, float eps, const ixb_cfg* cfg, ixb_stream stream);
 
+/* RMSNorm with an 8-bit output: h = x (+ res), rounded to the storage type;
+ * y = h * rsqrt(mean(h*h) + eps) * w in fp32; scales = max|y| / 448 over the row (group 0: scales[rows]) or
+ * over each 128 of its values (group 128: scales[rows, ceil(cols / 128)], the last over what is left);
+ * q[rows, cols] = e4m3(y / scale), to the nearest.  Where scale is 0 so is q; a NaN or an infinity of y
+ * makes its scale and what it covers NaN.  res and h_out may be null.  No counterpart in the reference: its norms
+ * leave 16 bits (inductor_x/lowering.py:217-233). */
+int ixb_rmsnorm_quantised(int dtype, const void* x, const void* res, const void* w, void* q,
+                          float* scales, void* h_out, int64_t rows, int64_t cols, int32_t group,
+                          float eps, ixb_stream stream);
+
 /* Reduce the last (stride-1) axis of contiguous x[rows, cols].
  * kind SUM/MEAN/AMAX/AMIN: out[rows] in x's dtype (fp32 accumulation, unlike the
  * reference's sum_ which always returns fp32, inductor_x/lowering.py:204-215).
@@ -268,6 +278,60 @@ int ixb_fa_bwd_scratch(int dtype, const void* q, const void* k, const void* v, c
                        const int64_t* dq_strides, const int64_t* dk_strides,
                        const int64_t* dv_strides, float scale, int causal, int32_t* status,
                        ixb_stream stream);
+
+/* ---- a decoder layer with a sliding window ------------------------------------------------ */
+
+/* Attention with a sliding window and first tokens that stay visible.  q[B,H,Sq,D], k/v[B,HK,Sk,D], o like q;
+ * H a multiple of HK: query head h reads key head h / (H / HK).  D = 128, dtype F16 or BF16, fp32 accumulation;
+ * strides and alignment as ixb_fa_fwd.  q_lengths and kv_lengths: int32[B] on the device or null (Sq and Sk;
+ * values outside [0, Sq] and [0, Sk] count as the nearest of those).  Query i of sequence b stands at position
+ * p = kv_lengths[b] - q_lengths[b] + i and sees key j when j <= p and (j > p - window or j < sinks) and
+ * j < kv_lengths[b]; a query that sees nothing, and any at or behind q_lengths[b], gets o = 0 and lse = -inf.
+ * lse[B,H,Sq] may be null.  window >= 1, 0 <= sinks <= 128, Sk >= 1, scale > 0 and finite.  `scratch` (16-byte
+ * aligned, contents lost) of ixb_window_attention_scratch_bytes bytes, which may be 0.  `status` as in
+ * ixb_fa_fwd.  The reference passes such bounds to the vendor kernel as pre_tockens / next_tockens
+ * (inductor_x/npu_fusion_attention_graph.py:13-18). */
+size_t ixb_window_attention_scratch_bytes(int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk,
+                                          int32_t window, int32_t sinks);
+int ixb_window_attention(int dtype, const void* q, const void* k, const void* v, void* o,
+                         float* lse, void* scratch, size_t scratch_bytes, int32_t B, int32_t H,
+                         int32_t HK, int32_t Sq, int32_t Sk, int32_t D, const int64_t* q_strides,
+                         const int64_t* k_strides, const int64_t* v_strides,
+                         const int64_t* o_strides, const int32_t* q_lengths,
+                         const int32_t* kv_lengths, float scale, int32_t window, int32_t sinks,
+                         int32_t* status, ixb_stream stream);
+
+/* Gradients of ixb_window_attention from its output `o` and log-sum-exp `lse`; dk and dv are summed over
+ * the query heads that share a key head.  Every element of dq, dk and dv is written: zeros where nothing
+ * was seen.  No atomics: the same bits every time.  `scratch` of ixb_window_attention_bwd_scratch_bytes
+ * bytes, 16-byte aligned, contents lost. */
+size_t ixb_window_attention_bwd_scratch_bytes(int32_t B, int32_t H, int32_t HK, int32_t Sq,
+                                              int32_t Sk, int32_t window, int32_t sinks);
+int ixb_window_attention_bwd(int dtype, const void* q, const void* k, const void* v, const void* o,
+                             const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                             void* scratch, size_t scratch_bytes, int32_t B, int32_t H, int32_t HK,
+                             int32_t Sq, int32_t Sk, int32_t D, const int64_t* q_strides,
+                             const int64_t* k_strides, const int64_t* v_strides,
+                             const int64_t* o_strides, const int64_t* do_strides,
+                             const int64_t* dq_strides, const int64_t* dk_strides,
+                             const int64_t* dv_strides, const int32_t* q_lengths,
+                             const int32_t* kv_lengths, float scale, int32_t window, int32_t sinks,
+                             int32_t* status, ixb_stream stream);
+
+/* Rotary positions with several axes, on q[B,heads,S,D] and k[B,k_heads,S,D] (either may have 0 heads; strides of
+ * the (batch, head, sequence) axes in elements, D contiguous; outputs with strides of their own, not overlapping
+ * the inputs); dtype F16, BF16 or F32, fp32 arithmetic.  sections[axes] (host memory): pairs of each axis, in
+ * order, at most 128 together and 2 * pairs <= D; frequencies[pairs] (host memory): radians a position.  Pair i of
+ * a head is turned by positions[axis(i), b, s] * frequencies[i], the angle formed in 64 bits; pair i is
+ * (i, pairs + i), or (2i, 2i + 1) with neighbours != 0; what lies behind the pairs is copied.  inverse != 0 turns the
+ * other way: the gradient.  positions I64 or I32 with the strides of its three axes in elements.  The reference has
+ * rotary embeddings as pointwise graphs only (inductor_x/lowering.py:45-88). */
+int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int64_t* q_strides,
+                     const int64_t* q_out_strides, int32_t heads, const void* k, void* k_out,
+                     const int64_t* k_strides, const int64_t* k_out_strides, int32_t k_heads,
+                     const void* positions, int position_dtype, const int64_t* position_strides,
+                     int32_t B, int32_t S, int32_t D, int32_t axes, const int32_t* sections,
+                     const double* frequencies, int neighbours, int inverse, ixb_stream stream);
 
 /* ---- context-parallel attention merge ---------------------------------------------------- */
 

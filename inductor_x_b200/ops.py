@@ -342,6 +342,236 @@ def fused_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     return dq, dk, dv
 
 
+# ---- a decoder layer with a sliding window -----------------------------------------------
+def rmsnorm_quantised(x, w, eps: float = 1e-6, *, residual=None, return_residual: bool = False, group: int = 0):
+    """RMSNorm over the last axis with an optional residual added first, and an 8-bit result.
+
+    Returns ``(q, scales)`` or ``(q, scales, h)``: ``h = x + residual`` rounded to the storage dtype, ``q``
+    (``torch.float8_e4m3fn``, the shape of ``x``) times ``scales`` (float32) the norm of ``h``.  ``group=0``: a scale
+    for each row, ``scales`` of shape ``x.shape[:-1]``; ``group=128``: one for each 128 values, ``[..., ceil(cols /
+    128)]``.  A scale is the largest magnitude / 448; the norm is rounded once, to 8 bits."""
+    _need_cuda(x, w, residual)
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if group not in (0, 128):
+        raise ValueError("group must be 0 (a scale a row) or 128")
+    if not x.is_contiguous() or x.dim() < 1:
+        raise ValueError("x must be contiguous")
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    if w.shape != (cols,) or w.dtype != x.dtype:
+        raise ValueError("w must be a vector of length cols in x's dtype")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
+                                 or not residual.is_contiguous()):
+        raise ValueError("residual must match x")
+    _one_device(x, w, residual)
+    w = w.contiguous()
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(x.shape[:-1] + ((-(-cols // group),) if group else ()), dtype=torch.float32, device=x.device)
+    h = torch.empty_like(x) if residual is not None and return_residual else None
+    if rows:
+        with torch.cuda.device(x.device):
+            rt.check("ixb_rmsnorm_quantised", rt.load().ixb_rmsnorm_quantised(
+                rt.DTYPE_CODE[x.dtype], x.data_ptr(), rt.ptr(residual), w.data_ptr(), q.data_ptr(), scales.data_ptr(),
+                rt.ptr(h), rows, cols, group, float(eps), rt.raw_stream(x.device)))
+    return (q, scales) if h is None else (q, scales, h)
+
+
+def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError("all tensors must be on one device")
+
+
+def _operand_strides(t: torch.Tensor):
+    """Strides of the (batch, head, sequence) axes; an axis of one entry, whose stride says nothing, counts as dense."""
+    B, H, S, D = t.shape
+    b, h, s, _ = t.stride()
+    s = s if S > 1 else D
+    h = h if H > 1 else S * D
+    return _I64x3(b if B > 1 else H * S * D, h, s)
+
+
+def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
+    _need_cuda(q, k, v, q_lengths, kv_lengths, *more)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("expected q[B,H,Sq,D], k[B,HK,Sk,D], v[B,HK,Sk,D]")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    if q.shape[3] != 128:
+        raise ValueError("the head dimension must be 128")
+    if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v, *more)):
+        raise ValueError("q, k, v (and out, dout) must share dtype float16 or bfloat16")
+    if not 1 <= window:
+        raise ValueError("window must be at least 1")
+    if not 0 <= sinks <= 128:
+        raise ValueError("sinks must be between 0 and 128")
+    for n in (q_lengths, kv_lengths):
+        if n is not None and (n.dtype != torch.int32 or n.shape != q.shape[:1]):
+            raise ValueError("lengths must be int32 [B]")
+    for t in (q, k, v, *more):
+        if t.numel() and t.stride(3) != 1:
+            raise ValueError("the head dimension must be contiguous")
+    _one_device(q, k, v, q_lengths, kv_lengths, *more)
+    most = 2 ** 31 - 1
+    return (min(int(window), most), int(sinks), q_lengths.contiguous() if q_lengths is not None else None,
+            kv_lengths.contiguous() if kv_lengths is not None else None)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, window: int, sinks: int = 0,
+                     q_lengths: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
+                     return_lse: bool = False, check: bool = False):
+    """Causal attention of ``q[B, H, Sq, D]`` over ``k``, ``v`` ``[B, HK, Sk, D]`` (``H`` a multiple of ``HK``, any
+    batch/head/sequence strides, ``D`` contiguous, ``D == 128``, fp16 or bf16) in which a query sees the last
+    ``window`` keys up to its own position and the first ``sinks`` (at most 128) of the sequence.
+
+    ``q_lengths`` and ``kv_lengths`` (int32 ``[B]`` on the device; all of ``Sq`` and ``Sk`` without) are the lengths of
+    a padded batch or of what a cache holds: query ``i`` stands at position ``kv_lengths[b] - q_lengths[b] + i``, the
+    last query at the last key.  A query that sees nothing, and any behind ``q_lengths[b]``, gets zeros and a
+    log-sum-exp of ``-inf``.  One to a few queries over a long cache are a decoding step: only the keys they see
+    are read.
+
+    Returns ``out`` (contiguous ``[B, H, Sq, D]``) or ``(out, lse)``; ``check=True`` as in :func:`fused_attention`."""
+    window, sinks, q_lengths, kv_lengths = _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths)
+    B, H, Sq, D = q.shape
+    HK, Sk = k.shape[1], k.shape[2]
+    out = torch.empty((B, H, Sq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device) if return_lse else None
+    if Sk == 0:  # nothing to see
+        out.zero_()
+        return (out, lse.fill_(float("-inf"))) if return_lse else out
+    status = torch.zeros(1, dtype=torch.int32, device=q.device) if check else None
+    lib = rt.load()
+    room = lib.ixb_window_attention_scratch_bytes(B, H, HK, Sq, Sk, window, sinks)
+    scratch = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
+    with torch.cuda.device(q.device):
+        rt.check("ixb_window_attention", lib.ixb_window_attention(
+            rt.DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rt.ptr(lse), rt.ptr(scratch),
+            room, B, H, HK, Sq, Sk, D, _operand_strides(q), _operand_strides(k), _operand_strides(v), _operand_strides(out),
+            rt.ptr(q_lengths), rt.ptr(kv_lengths), float(scale), window, sinks, rt.ptr(status), rt.raw_stream(q.device)))
+    if status is not None and int(status.item()) != 0:
+        raise RuntimeError("ixb_window_attention: an internal pipeline wait gave up; output is undefined")
+    return (out, lse) if return_lse else out
+
+
+def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
+                              dout: torch.Tensor, scale: float, *, window: int, sinks: int = 0,
+                              q_lengths: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
+                              check: bool = False):
+    """Gradients ``(dq, dk, dv)`` of :func:`window_attention` from its inputs, its output ``out``, its log-sum-exp
+    ``lse`` (``return_lse=True``) and the incoming gradient ``dout``; ``dk`` and ``dv`` are sums over the query heads
+    that share a key head, and zero where no query sees the key.  Deterministic, no atomics."""
+    window, sinks, q_lengths, kv_lengths = _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths)
+    _need_cuda(out, lse, dout)
+    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype:
+        raise ValueError("out and dout must have the shape and dtype of q")
+    B, H, Sq, D = q.shape
+    HK, Sk = k.shape[1], k.shape[2]
+    if lse.shape != (B, H, Sq) or lse.dtype != torch.float32:
+        raise ValueError("lse must be float32 [B, H, Sq]")
+    _one_device(q, out, lse, dout)
+    lse = lse.contiguous()
+    if dout.numel() and (dout.stride(3) != 1 or any(st <= 0 or st % 8 for st in _operand_strides(dout))):
+        dout = dout.contiguous()
+    if out.numel() and out.stride(3) != 1:
+        raise ValueError("the head dimension must be contiguous")
+    dq = torch.empty((B, H, Sq, D), dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty((B, HK, Sk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+    if Sq == 0 or Sk == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    status = torch.zeros(1, dtype=torch.int32, device=q.device) if check else None
+    lib = rt.load()
+    room = lib.ixb_window_attention_bwd_scratch_bytes(B, H, HK, Sq, Sk, window, sinks)
+    scratch = torch.empty(room, dtype=torch.uint8, device=q.device)
+    like_q, like_k = _operand_strides(dq), _operand_strides(dk)
+    with torch.cuda.device(q.device):
+        rt.check("ixb_window_attention_bwd", lib.ixb_window_attention_bwd(
+            rt.DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), scratch.data_ptr(), room, B, H, HK, Sq, Sk, D, _operand_strides(q),
+            _operand_strides(k), _operand_strides(v), _operand_strides(out), _operand_strides(dout), like_q, like_k, like_k,
+            rt.ptr(q_lengths), rt.ptr(kv_lengths), float(scale), window, sinks, rt.ptr(status), rt.raw_stream(q.device)))
+    if status is not None and int(status.item()) != 0:
+        raise RuntimeError("ixb_window_attention_bwd: an internal pipeline wait gave up; gradients are undefined")
+    return dq, dk, dv
+
+
+PAIRINGS, LADDERS = ("halves", "neighbours"), ("shared", "own")
+
+
+@functools.lru_cache(maxsize=256)
+def _rotary_plan(sections: tuple, base: float, ladder: str, frequencies: Optional[tuple]):
+    """(pairs, axes, ctypes sections, ctypes frequencies in radians a position)."""
+    pairs = sum(sections)
+    if not sections or any(n < 0 for n in sections) or not 1 <= pairs <= 128:
+        raise ValueError("sections must be one count of pairs for each axis, 1 to 128 together")
+    if frequencies is None:
+        if not base > 0:
+            raise ValueError("base must be positive")
+        powers = [j / n for n in sections for j in range(n)] if ladder == "own" else [i / pairs for i in range(pairs)]
+        frequencies = tuple(base ** -p for p in powers)
+    if len(frequencies) != pairs:
+        raise ValueError("frequencies must be one number for each pair")
+    return pairs, len(sections), (ctypes.c_int32 * len(sections))(*sections), (ctypes.c_double * pairs)(*frequencies)
+
+
+def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inverse):
+    _need_cuda(q, k, positions)
+    if pairing not in PAIRINGS or ladder not in LADDERS:
+        raise ValueError(f"pairing must be one of {PAIRINGS}, ladder one of {LADDERS}")
+    pairs, axes, c_sections, c_frequencies = _rotary_plan(
+        tuple(sections), float(base), ladder, tuple(frequencies) if frequencies is not None else None)
+    if q.dtype not in (torch.float32, torch.float16, torch.bfloat16) or (k is not None and k.dtype != q.dtype):
+        raise ValueError("q and k must share dtype float32, float16 or bfloat16")
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
+        raise ValueError("expected q[B,H,S,D], k[B,HK,S,D]")
+    B, H, S, D = q.shape
+    if 2 * pairs > D:
+        raise ValueError("the sections turn more than the head dimension has")
+    if positions.dtype not in (torch.int64, torch.int32) or positions.shape not in ((axes, B, S), (axes, S)):
+        raise ValueError("positions must be int32 or int64 [axes, B, S] or [axes, S]")
+    if any(t is not None and t.numel() and t.stride(3) != 1 for t in (q, k)):
+        raise ValueError("the head dimension must be contiguous")
+    _one_device(q, k, positions)
+    at = positions.stride() if positions.dim() == 3 else (positions.stride(0), 0, positions.stride(1))
+    # (an expanded input's result is a dense tensor of its own)
+    new = lambda t: torch.empty_like(t) if all(t.stride()) else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    q_out, k_out = new(q), None if k is None else new(k)
+    strides = lambda t: _I64x3(*t.stride()[:3]) if t is not None else None  # noqa: E731
+    if q.numel() or (k is not None and k.numel()):
+        with torch.cuda.device(q.device):
+            rt.check("ixb_axial_rotary", rt.load().ixb_axial_rotary(
+                rt.DTYPE_CODE[q.dtype], q.data_ptr(), q_out.data_ptr(), strides(q), strides(q_out), H, rt.ptr(k), rt.ptr(k_out),
+                strides(k), strides(k_out), k.shape[1] if k is not None else 0, positions.data_ptr(),
+                rt.DTYPE_CODE[positions.dtype], _I64x3(*at), B, S, D, axes, c_sections, c_frequencies,
+                int(pairing == "neighbours"), int(inverse), rt.raw_stream(q.device)))
+    return q_out if k is None else (q_out, k_out)
+
+
+def axial_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, sections: Sequence[int], *,
+                 base: float = 10000.0, pairing: str = "halves", ladder: str = "shared",
+                 frequencies: Optional[Sequence[float]] = None):
+    """Rotary positions with one or several axes (time, height, width) on ``q[B, H, S, D]`` and ``k[B, HK, S, D]`` (any
+    batch/head/sequence strides, ``D`` contiguous; fp32, fp16 or bf16; ``k`` may be None).
+
+    ``positions`` (int32 or int64) is ``[axes, B, S]`` or, the same for every sequence, ``[axes, S]``;
+    ``sections`` says how many pairs each axis turns, in order.  Pair ``i`` is turned by its axis' position times its
+    frequency: ``base ** -(i / pairs)`` along one ladder over all pairs (``ladder="shared"``), ``base ** -(j / n)`` for
+    pair ``j`` of an axis of ``n`` (``"own"``), or ``frequencies[i]``.  ``pairing="halves"`` pairs ``i`` with ``i +
+    pairs``, ``"neighbours"`` ``2 i`` with ``2 i + 1``.  What lies behind the pairs is copied.  Angles are formed in 64
+    bits, so that far positions keep their fraction of a turn.
+
+    Returns the turned ``(q, k)``, or ``q`` alone where ``k`` is None, in the memory order of the inputs."""
+    return _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, False)
+
+
+def axial_rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], positions: torch.Tensor, sections: Sequence[int], *,
+                          base: float = 10000.0, pairing: str = "halves", ladder: str = "shared",
+                          frequencies: Optional[Sequence[float]] = None):
+    """Gradients of :func:`axial_rotary` for its ``q`` and ``k`` from those of its results: the same turns the other
+    way."""
+    return _rotary(dq, dk, positions, sections, base, pairing, ladder, frequencies, True)
+
+
 # ---- context-parallel attention merge ----------------------------------------------------
 def _stat_nstride(t: torch.Tensor, S: int) -> int:
     """Element stride of the N axis of a ``[B, N, S, 8]`` statistics tensor whose last two

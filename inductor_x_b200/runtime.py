@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from typing import Optional
 
 import torch
@@ -109,6 +109,16 @@ _SIGNATURES = {
     "ixb_fa_bwd_scratch_bytes": (c_size_t, [c_int32] * 4 + [c_int, c_size_t]),
     "ixb_fa_bwd_scratch": (c_int, [c_int] + [c_void_p] * 11 + [c_size_t] + [c_int32] * 5 + [POINTER(c_int64)] * 8 +
                            [c_float, c_int, c_void_p, c_void_p]),
+    "ixb_rmsnorm_quantised": (c_int, [c_int] + [c_void_p] * 6 + [c_int64] * 2 + [c_int32, c_float, c_void_p]),
+    "ixb_window_attention_scratch_bytes": (c_size_t, [c_int32] * 7),
+    "ixb_window_attention": (c_int, [c_int] + [c_void_p] * 6 + [c_size_t] + [c_int32] * 6 + [POINTER(c_int64)] * 4 +
+                             [c_void_p] * 2 + [c_float, c_int32, c_int32, c_void_p, c_void_p]),
+    "ixb_window_attention_bwd_scratch_bytes": (c_size_t, [c_int32] * 7),
+    "ixb_window_attention_bwd": (c_int, [c_int] + [c_void_p] * 10 + [c_size_t] + [c_int32] * 6 + [POINTER(c_int64)] * 8 +
+                                 [c_void_p] * 2 + [c_float, c_int32, c_int32, c_void_p, c_void_p]),
+    "ixb_axial_rotary": (c_int, [c_int] + [c_void_p, c_void_p, POINTER(c_int64), POINTER(c_int64), c_int32] * 2 +
+                         [c_void_p, c_int, POINTER(c_int64)] + [c_int32] * 4 +
+                         [POINTER(c_int32), POINTER(c_double), c_int, c_int, c_void_p]),
     "ixb_index_select_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                       c_int, c_int, c_void_p, c_void_p]),
     "ixb_cp_forward_update": (c_int, [c_int] + [c_void_p] * 9 + [c_int32] * 4 + [c_int64] * 3 + [c_void_p]),
