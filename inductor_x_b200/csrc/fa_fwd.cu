@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (p.causal && qi + diag < last) last = qi + diag;
           lim = last - col0;
         }
-        softmax_tile<IS_BF16>(s_addr, o_addr, edge, lim, j == 0, p.scale_log2, m_used, l, &p_full[t], &p_rest[t]);
+        softmax_tile<IS_BF16>(s_addr, o_addr, CausalMask{edge, lim}, j == 0, p.scale_log2, m_used, l, &p_full[t], &p_rest[t]);
         ++seen;
       }
       if (ok && my_n_kv > 0) {

@@ -27,14 +27,14 @@ inline EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-// dims (d, s, h, b); strides in elements; rows past S are zero-filled by the copy engine
+// dims (d, s, h, b); strides in elements; rows past S are zero-filled by the copy engine; a box of `rows` rows
 inline int make_fa_map(CUtensorMap* map, const void* base, int is_bf16, int B, int H, int S, long long sb,
-                       long long sh, long long ss) {
+                       long long sh, long long ss, int rows = 128) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return IXB_ERR_CUDA;
   const cuuint64_t dims[4] = {128, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  const cuuint32_t box[4] = {64, 128, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   auto encode = [&] {
     return fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.causal && qi + diag < last) last = qi + diag;
         lim = last - col0;
       }
-      softmax_tile<IS_BF16>(s_addr, o_addr, edge, lim, k == 0, p.scale_log2, m_used, l, &p_full[t_own], &p_rest[t_own]);
+      softmax_tile<IS_BF16>(s_addr, o_addr, CausalMask{edge, lim}, k == 0, p.scale_log2, m_used, l, &p_full[t_own], &p_rest[t_own]);
     }
     if (ok && mine > 0) ok = __all_sync(kFull, mbar_wait(&pv_done[t_own], 0, &failed));  // the slot's last product
     if (!ok && lane == 0) failed = 1;

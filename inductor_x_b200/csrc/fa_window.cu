@@ -4,7 +4,7 @@
 //   out = softmax(scale q k^T) v over what it sees, lse its log-sum-exp (no key: 0 and -inf).
 // H query heads share HK key heads, H / HK neighbours each.
 #include <cmath>
-#include "fa_maps.h"
+#include "fa_window.h"
 #include "ixb/tcgen05.cuh"
 
 namespace {
@@ -52,33 +52,6 @@ __device__ __forceinline__ Lengths lengths_of(const WinParams& p, int b) {
   n.q = p.q_lengths ? min(max(p.q_lengths[b], 0), p.Sq) : p.Sq;
   n.kv = p.kv_lengths ? min(max(p.kv_lengths[b], 0), p.Sk) : p.Sk;
   return n;
-}
-
-// a warp a query row
-template <class T> __global__ void window_fwd_kernel(const WinParams p) {
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= (long long)p.B * p.H * p.Sq) return;
-  const int b = (int)(row / ((long long)p.H * p.Sq)), h = (int)(row / p.Sq % p.H), i = (int)(row % p.Sq);
-  const Lengths n = lengths_of(p, b);
-  const int at = n.kv - n.q + i;
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (i < n.q && at >= 0) {
-    const float4 q = row4<T>(p.q, b, h, i, lane);
-    const int hk = h / (p.H / p.HK), low = max(0, at - p.window + 1);
-    for (int j = 0; j <= at; ++j) {
-      if (j < low && j >= p.sinks) j = low;
-      const float s = dot(q, row4<T>(p.k, b, hk, j, lane)) * p.scale;
-      const float top = fmaxf(m, s), f = m == -INFINITY ? 0.f : expf(m - top), e = expf(s - top);
-      l = l * f + e;
-      acc = axpy(e, row4<T>(p.v, b, hk, j, lane), make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-      m = top;
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  put4<T>(p.o, b, h, i, lane, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-  if (lane == 0 && p.lse != nullptr) p.lse[row] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 // a warp a query row: dq
@@ -133,53 +106,22 @@ template <class T> __global__ void window_dkv_kernel(const WinParams p, const fl
 
 View view_of(const void* ptr, const int64_t* strides) { return View{ptr, strides[0], strides[1], strides[2]}; }
 
-int check_operands(int n, const void* const* ptrs, const int64_t* const* strides) {
-  for (int t = 0; t < n; ++t) {
-    if (ptrs[t] == nullptr || strides[t] == nullptr) return IXB_ERR_ARG;
-    if (!ixb_host::aligned16(ptrs[t])) return IXB_ERR_ALIGN;
-    for (int i = 0; i < 3; ++i)
-      if (strides[t][i] <= 0 || strides[t][i] % 8 != 0) return IXB_ERR_ALIGN;
-  }
-  return IXB_OK;
-}
-
-int check_sizes(int dtype, int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk, int32_t D, float scale, int32_t window,
-                int32_t sinks) {
-  if (B < 0 || H < 0 || HK < 0 || Sq < 0 || Sk < 0 || window < 1 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return IXB_ERR_ARG;
-  if (dtype != IXB_BF16 && dtype != IXB_F16) return IXB_ERR_DTYPE;
-  if (D != HD || (HK == 0 ? H != 0 : H % HK != 0) || sinks > 128) return IXB_ERR_SHAPE;
-  return IXB_OK;
-}
-
 }  // namespace
 
 extern "C" size_t ixb_window_attention_scratch_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
 
 extern "C" int ixb_window_attention(int dtype, const void* q, const void* k, const void* v, void* o, float* lse, void*,
-                                    size_t, int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk, int32_t D, const int64_t* q_strides,
-                                    const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
-                                    const int32_t* q_lengths, const int32_t* kv_lengths, float scale, int32_t window,
-                                    int32_t sinks, int32_t* status, ixb_stream stream) {
-  if (int st = check_sizes(dtype, B, H, HK, Sq, Sk, D, scale, window, sinks)) return st;
+                                    size_t, int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk, int32_t D,
+                                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                    const int64_t* o_strides, const int32_t* q_lengths, const int32_t* kv_lengths, float scale,
+                                    int32_t window, int32_t sinks, int32_t* status, ixb_stream stream) {
+  if (int st = ixb_host::check_window_sizes(dtype, B, H, HK, Sq, Sk, D, scale, window, sinks)) return st;
   if (B == 0 || H == 0 || Sq == 0) return IXB_OK;
   if (Sk == 0) return IXB_ERR_SHAPE;
-  const void* ptrs[] = {q, k, v, o};
-  const int64_t* strs[] = {q_strides, k_strides, v_strides, o_strides};
-  if (int st = check_operands(4, ptrs, strs)) return st;
-  WinParams p = {};
-  p.q = view_of(q, q_strides);
-  p.k = view_of(k, k_strides);
-  p.v = view_of(v, v_strides);
-  p.o = view_of(o, o_strides);
-  p.lse = lse;
-  p.q_lengths = q_lengths;
-  p.kv_lengths = kv_lengths;
-  p.B = B, p.H = H, p.HK = HK, p.Sq = Sq, p.Sk = Sk;
-  p.scale = scale, p.window = window, p.sinks = sinks;
-  const unsigned grid = (unsigned)(((long long)B * H * Sq + 7) / 8);
-  if (dtype == IXB_BF16) window_fwd_kernel<bf16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  else window_fwd_kernel<f16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  return ixb_host::cuda_status(cudaGetLastError());
+  const ixb_host::WindowView views[] = {{q, q_strides}, {k, k_strides}, {v, v_strides}, {o, o_strides}};
+  if (int st = ixb_host::check_window_views(views, 4)) return st;
+  const ixb_host::WindowShape a{dtype == IXB_BF16, B, H, HK, Sq, Sk, q_lengths, kv_lengths, scale, window < Sk ? window : Sk, sinks};
+  return ixb_host::window_prefill(a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
 }
 
 extern "C" size_t ixb_window_attention_bwd_scratch_bytes(int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk,
@@ -196,12 +138,12 @@ extern "C" int ixb_window_attention_bwd(int dtype, const void* q, const void* k,
                                         const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
                                         const int32_t* q_lengths, const int32_t* kv_lengths, float scale, int32_t window,
                                         int32_t sinks, int32_t* status, ixb_stream stream) {
-  if (int st = check_sizes(dtype, B, H, HK, Sq, Sk, D, scale, window, sinks)) return st;
+  if (int st = ixb_host::check_window_sizes(dtype, B, H, HK, Sq, Sk, D, scale, window, sinks)) return st;
   if (B == 0 || H == 0) return IXB_OK;
   if (Sq == 0 || Sk == 0) return IXB_ERR_SHAPE;
-  const void* ptrs[] = {q, k, v, o, dout, dq, dk, dv};
-  const int64_t* strs[] = {q_strides, k_strides, v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides};
-  if (int st = check_operands(8, ptrs, strs)) return st;
+  const ixb_host::WindowView views[] = {{q, q_strides},   {k, k_strides},   {v, v_strides},   {o, o_strides}, {dout, do_strides},
+                                        {dq, dq_strides}, {dk, dk_strides}, {dv, dv_strides}};
+  if (int st = ixb_host::check_window_views(views, 8)) return st;
   if (lse == nullptr) return IXB_ERR_ARG;
   if (scratch == nullptr || scratch_bytes < ixb_window_attention_bwd_scratch_bytes(B, H, HK, Sq, Sk, window, sinks)) return IXB_ERR_SCRATCH;
   if (!ixb_host::aligned16(scratch)) return IXB_ERR_ALIGN;

@@ -1,0 +1,482 @@
+// Attention with a sliding window and first tokens that stay visible, forward, on tcgen05 tensor cores (the meaning of
+// the arguments: fa_window.h).  The pipeline is that of fa_fwd.cu - TMA producer, MMA issuer, scheduler, two warpgroups
+// of softmax, running blocks that take over pending items - on other work items:
+//
+// A tile of 128 rows is R rows of each of 128 / R neighbouring query heads that share a key head: R is 128, or the
+// power of two that holds all of the call's queries where they are fewer (8 at least).  The tiles of a key
+// head, those of the same rows one after the other, go two to an item, so that with an even number of
+// sharing heads both tiles of an item see the very same keys and every tile of K and V serves both.
+// An item walks the first key tile, where it is not in the window but has first tokens, and the key tiles from the
+// one its window begins in to the one its last row stands in.  A tile of rows leaves out those that only the other one sees.
+//
+// What lies behind a sequence's length in K and V may be anything: scores of hidden keys are replaced before they are
+// looked at, but a probability of 0 times a NaN is one, so the producer clears the rows of V behind the length in the
+// tile that holds it.
+#include <atomic>
+#include "fa_window.h"
+#include "ixb/fa_softmax.cuh"
+
+namespace {
+
+using namespace ixb;
+using namespace ixb::fa;
+
+constexpr int kStages = 2;  // (the issuer picks stage descriptors with two-way selects)
+// Registers: as in fa_fwd.cu
+constexpr int kRegsLaunch = 168, kRegsIssue = 80, kRegsSoftmax = 208;
+static_assert(kRegsIssue + NQ * kRegsSoftmax <= (1 + NQ) * kRegsLaunch, "setmaxnreg draws on the block's own registers");
+constexpr size_t kSmemBytes = (size_t)kTileBytes * (NQ + 2 * kStages) + 1024;
+
+struct WinParams {
+  void* o;
+  float* lse;            // [B, H, Sq], may be null
+  int* status;           // may be null
+  const int *q_lengths, *kv_lengths;
+  long long o_stride_b, o_stride_h, o_stride_s;  // elements
+  int B, H, HK, share, Sq, Sk;
+  float scale_log2;
+  int window, sinks;
+  int rows_log2;         // R = 1 << rows_log2 rows of a head in a tile
+  int tiles;             // tiles of rows a key head has
+  int wide;
+};
+
+// Of a row at position `at`: keys of the tile behind `lim` are hidden, and those in [from, low), the ones between the first
+// tokens and the window.
+struct WindowMask {
+  bool edge;
+  int lim, from, low;
+  __device__ __forceinline__ void apply(uint32_t (&raw)[BN]) const {
+    if (!edge) return;
+    // the first n keys of 32
+    auto first = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
+#pragma unroll
+    for (int c = 0; c < BN / 32; ++c) {
+      const uint32_t seen = first(lim + 1 - c * 32) & ~(first(low - c * 32) & ~first(from - c * 32));
+      if (__all_sync(kFull, seen == 0xffffffffu)) continue;
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (!(seen >> e & 1u)) raw[c * 32 + e] = 0xff800000u;  // -inf
+    }
+  }
+};
+
+template <bool IS_BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    fa_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const WinParams p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* q_smem = smem;
+  unsigned char* k_smem = smem + kTileBytes * NQ;
+  unsigned char* v_smem = smem + kTileBytes * (NQ + kStages);
+
+  __shared__ __align__(16) uint4 next_answer[2];
+  __shared__ __align__(8) uint64_t q_full, q_empty, next_wanted, next_full[2], next_taken[2], k_full[kStages],
+      k_empty[kStages], v_full[kStages], v_empty[kStages], v_raw, s_full[NQ], p_full[NQ], p_rest[NQ], pv_done[NQ], drained;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ volatile int failed;
+
+  const int warp = __shfl_sync(kFull, (int)threadIdx.x >> 5, 0);  // known uniform to the compiler
+  const int lane = threadIdx.x & 31;
+
+  const int R = 1 << p.rows_log2, blocks_of_heads = (p.share + (BM >> p.rows_log2) - 1) >> (7 - p.rows_log2);
+  struct Item {
+    int b, hk, off, q_len, kv_len;   // query i stands at position off + i
+    int i0[NQ], h0[NQ];              // first row and first head of each tile (h0 < 0: no such tile)
+    int lo[NQ], hi[NQ];              // key tiles of each tile's window (none: hi = 0)
+    int lo_all, n_kv, first;         // first: the walk begins with key tile 0, which is in no window
+  };
+  auto item_of = [&](int index) {
+    Item w;
+    const int per_head = (p.tiles + NQ - 1) / NQ;
+    const int bh = index / per_head, n = per_head - 1 - (index - bh * per_head);  // late (long) ones of a head first
+    w.b = bh / p.HK;
+    w.hk = bh - w.b * p.HK;
+    w.q_len = p.q_lengths != nullptr ? min(max(__ldg(p.q_lengths + w.b), 0), p.Sq) : p.Sq;
+    w.kv_len = p.kv_lengths != nullptr ? min(max(__ldg(p.kv_lengths + w.b), 0), p.Sk) : p.Sk;
+    w.off = w.kv_len - w.q_len;
+    w.lo_all = 1 << 30;
+    int end = 0;
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      const int u = NQ * n + t, i = u / blocks_of_heads;
+      w.i0[t] = i * BM;  // (fewer rows a head than a tile has: all of them are in tile 0)
+      w.h0[t] = u < p.tiles ? w.hk * p.share + ((u - i * blocks_of_heads) << (7 - p.rows_log2)) : -1;
+      const int last = w.off + min(w.i0[t] + R, w.q_len) - 1;  // position of the tile's last row, and of its first
+      const int begin = max(w.off + w.i0[t], 0);
+      const bool any = u < p.tiles && w.i0[t] < w.q_len && last >= 0;
+      w.lo[t] = any ? max(begin - p.window + 1, 0) / BN : 0;
+      w.hi[t] = any ? last / BN + 1 : 0;
+      if (any) {
+        w.lo_all = min(w.lo_all, w.lo[t]);
+        end = max(end, w.hi[t]);
+      }
+    }
+    w.first = end > 0 && w.lo_all > 0 && p.sinks > 0 ? 1 : 0;
+    w.n_kv = end > 0 ? end - w.lo_all + w.first : 0;
+    return w;
+  };
+  // key tile of step x of an item, and whether tile t of rows looks at it
+  auto key_tile = [&](const Item& w, int x) { return w.first ? (x == 0 ? 0 : w.lo_all + x - 1) : w.lo_all + x; };
+  auto looks = [&](const Item& w, int t, int x) {
+    if (x >= w.n_kv) return false;
+    const int j = key_tile(w, x);
+    const int lo = t ? w.lo[1] : w.lo[0], hi = t ? w.hi[1] : w.hi[0];
+    return hi > 0 && j < hi && (j >= lo || (j == 0 && p.sinks > 0));
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
+    mbar_init(&next_wanted, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&next_full[s], 1);
+      mbar_init(&next_taken[s], 2 + NQ * 4);  // producer, issuer and the softmax warps
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(&v_raw, 1);
+    for (int t = 0; t < NQ; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 128);
+      mbar_init(&p_rest[t], 128);
+      mbar_init(&pv_done[t], 1);
+    }
+    mbar_init(&drained, 1);
+    failed = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) tc::tmem_alloc(&tmem_base_slot, kTmemCols);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem_base = tmem_base_slot;
+
+  // The item after item n of this block: answer n of the scheduler warp.  Taken by a whole warp.
+  auto take_next = [&](int n, bool& ok) {
+    ok = ok && __all_sync(kFull, mbar_wait(&next_full[n & 1], (n >> 1) & 1, &failed));
+    if (!ok) return -1;
+    const int index = __shfl_sync(kFull, tc::next_block(&next_answer[n & 1]), 0);
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&next_taken[n & 1]);
+    return index;
+  };
+
+  int q_loads = 0, k_loads = 0, v_loads = 0, raw_loads = 0;  // producer: what it has asked for
+  bool raw_pending = false;                                  // the last copy of V completes v_raw, not v_full
+  int asked = 0;                                             // scheduler: the same
+  if (warp < 4) {
+    tc::regs_dec<kRegsIssue>();
+    if (warp == 0) {
+      // ------------------------------------------------------------------ TMA producer
+      bool ok = true;
+      int step = 0;  // key tiles loaded so far, over all items
+      for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
+        const Item w = item_of(index);
+        if (w.n_kv > 0) {
+          ok = q_loads == 0 || __all_sync(kFull, mbar_wait(&q_empty, (q_loads - 1) & 1, &failed));
+          if (!ok) break;
+          if (lane == 0) {
+            // rows and heads past the end of the tensor are zero-filled by the copy engine (a head behind the key head's own
+            // is another one's: its rows are not stored)
+            mbar_arrive_expect_tx(&q_full, kTileBytes * NQ);
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) {
+              unsigned char* qd = q_smem + t * kTileBytes;
+              const int h0 = max(w.h0[t], 0);
+              for (int g = 0; g < BM >> p.rows_log2; ++g, qd += R * 128) {
+                tc::tma_load_4d(qd, &map_q, &q_full, 0, w.i0[t], h0 + g, w.b);
+                tc::tma_load_4d(qd + kHalfBytes, &map_q, &q_full, 64, w.i0[t], h0 + g, w.b);
+              }
+            }
+          }
+          ++q_loads;
+        }
+        for (int x = 0; x < w.n_kv; ++x, ++step) {
+          const int s = step & 1, u = step >> 1, j = key_tile(w, x);
+          ok = u == 0 || __all_sync(kFull, mbar_wait(&k_empty[s], (u - 1) & 1, &failed));
+          if (!ok) break;
+          if (lane == 0) {
+            unsigned char* kd = k_smem + (size_t)s * kTileBytes;
+            mbar_arrive_expect_tx(&k_full[s], kTileBytes);
+            tc::tma_load_4d(kd, &map_k, &k_full[s], 0, j * BN, w.hk, w.b);
+            tc::tma_load_4d(kd + kHalfBytes, &map_k, &k_full[s], 64, j * BN, w.hk, w.b);
+            if (x + 1 == w.n_kv) tc::mbar_arrive(&next_wanted);
+          }
+          k_loads = step + 1;
+          ok = u == 0 || __all_sync(kFull, mbar_wait(&v_empty[s], (u - 1) & 1, &failed));
+          if (!ok) break;
+          unsigned char* vd = v_smem + (size_t)s * kTileBytes;
+          const int live = w.kv_len - j * BN;
+          const bool clear = live < BN && w.kv_len < p.Sk;  // the tile reaches behind the sequence, and not behind the tensor
+          uint64_t* bar = clear ? &v_raw : &v_full[s];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, kTileBytes);
+            tc::tma_load_4d(vd, &map_v, bar, 0, j * BN, w.hk, w.b);
+            tc::tma_load_4d(vd + kHalfBytes, &map_v, bar, 64, j * BN, w.hk, w.b);
+          }
+          if (clear) {
+            raw_pending = true;
+            ok = __all_sync(kFull, mbar_wait(&v_raw, raw_loads & 1, &failed));
+            ++raw_loads;
+            if (!ok) break;
+            raw_pending = false;
+            // a row is 128 bytes in each of the two boxes, whichever way its pieces are swizzled
+            for (int at = live * 8 + lane; at < BN * 8; at += 32) {
+              *reinterpret_cast<uint4*>(vd + at * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(vd + kHalfBytes + at * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&v_full[s]);
+          }
+          v_loads = step + 1;
+        }
+        if (ok && w.n_kv == 0 && lane == 0) tc::mbar_arrive(&next_wanted);
+        __syncwarp();
+        index = take_next(n, ok);
+      }
+      if (!ok && lane == 0) failed = 1;
+    } else if (warp == 1) {
+      // -------------------------------------------------------------------- MMA issuer
+      // The whole warp runs this role and an elected lane issues (see tc::product_ss).
+      constexpr uint32_t idesc_qk = tc::instr_desc(BM, BN, IS_BF16 ? 1 : 0, 0, 0);
+      constexpr uint32_t idesc_pv = tc::instr_desc(BM, HD, IS_BF16 ? 1 : 0, 0, 1);
+      const uint32_t tmem = __shfl_sync(kFull, tmem_base, 0);
+      const uint64_t q_desc = tc::smem_desc(smem_u32(q_smem), 16, 1024);
+      const uint64_t k_desc = tc::smem_desc(smem_u32(k_smem), 16, 1024);
+      const uint64_t v_desc = tc::smem_desc(smem_u32(v_smem), kHalfBytes, 1024);
+      // tile t, stage s: the address field moves by whole tiles and cannot carry out of it
+      auto issue_qk = [&](int t, int stage) {
+        tc::product_ss<kHalfBytes>(tmem + kColS + t * 128, q_desc + (uint32_t)(t * (kTileBytes >> 4)),
+                                   k_desc + (uint32_t)(stage * (kTileBytes >> 4)), idesc_qk);
+        tc::commit_elected(&s_full[t]);
+      };
+      bool ok = true;
+      int step = 0;               // key tiles consumed so far, over all items
+      int items = 0;              // items with keys so far
+      int products[NQ] = {0, 0};  // P tiles consumed so far
+      for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
+        const Item w = item_of(index);
+        if (w.n_kv > 0) {
+          ok = __all_sync(kFull, mbar_wait(&q_full, items & 1, &failed)) &&
+               __all_sync(kFull, mbar_wait(&k_full[step & 1], (step >> 1) & 1, &failed));
+          if (!ok) break;
+          ++items;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int t = 0; t < NQ; ++t)
+            if (looks(w, t, 0)) issue_qk(t, step & 1);
+          tc::commit_elected(&k_empty[step & 1]);
+          if (w.n_kv == 1) tc::commit_elected(&q_empty);
+        }
+        bool begun[NQ] = {false, false};
+        for (int x = 0; x < w.n_kv; ++x) {
+          const int s = (step + x) & 1, u = (step + x) >> 1;
+          const int s1 = (step + x + 1) & 1, u1 = (step + x + 1) >> 1;
+          ok = __all_sync(kFull, mbar_wait(&v_full[s], u & 1, &failed));
+          if (x + 1 < w.n_kv) ok = ok && __all_sync(kFull, mbar_wait(&k_full[s1], u1 & 1, &failed));
+          if (!ok) break;
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            const bool do_qk = looks(w, t, x + 1);
+            if (looks(w, t, x)) {
+              // O_t += P_t V_j in two parts, as in fa_fwd.cu
+              ok = ok && __all_sync(kFull, mbar_wait(&p_full[t], products[t] & 1, &failed));
+              if (!ok) break;
+              tc::fence_after_sync();
+              const uint64_t vd = v_desc + (uint32_t)(s * (kTileBytes >> 4));
+              const uint32_t o = tmem + kColO + t * 128, pa = tmem + kColS + t * 128;
+              tc::product_ts<kSplit / 16>(o, pa, vd, idesc_pv, begun[t]);
+              ok = __all_sync(kFull, mbar_wait(&p_rest[t], products[t] & 1, &failed));
+              if (!ok) break;
+              tc::fence_after_sync();
+              // (16 keys of V are 2048 bytes of a 64-column box)
+              tc::product_ts<(BN - kSplit) / 16>(o, pa + kSplit / 2, vd + (uint32_t)(kSplit / 16 * 2048 >> 4), idesc_pv, 1u);
+              ++products[t];
+              begun[t] = true;
+              // the tile's last product: the key tile that its last row stands in
+              if (key_tile(w, x) + 1 == (t ? w.hi[1] : w.hi[0])) tc::commit_elected(&pv_done[t]);
+            }
+            // P_t has been consumed by the MMAs just issued (the tensor core runs them in
+            // order), so tile t's buffer can take the scores of the next step
+            if (do_qk) issue_qk(t, s1);
+          }
+          if (!ok) break;
+          tc::commit_elected(&v_empty[s]);
+          if (x + 1 < w.n_kv) tc::commit_elected(&k_empty[s1]);
+          if (x + 2 == w.n_kv) tc::commit_elected(&q_empty);  // the item's last scores are issued
+        }
+        step += w.n_kv;
+        index = take_next(n, ok);
+      }
+      if (!ok && lane == 0) failed = 1;
+      __syncwarp();
+    } else if (warp == 2) {
+      // -------------------------------------------------------------------- scheduler (as in fa_fwd.cu)
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        ok = __all_sync(kFull, mbar_wait(&next_wanted, n & 1, &failed));
+        if (ok && n > 0) ok = __all_sync(kFull, mbar_wait(&next_taken[(n - 1) & 1], ((n - 1) >> 1) & 1, &failed));
+        if (!ok) break;
+        if (lane == 0) tc::request_next_block(&next_answer[n & 1], &next_full[n & 1]);
+        asked = n + 1;
+        ok = __all_sync(kFull, mbar_wait(&next_full[n & 1], (n >> 1) & 1, &failed));
+        if (!ok || __shfl_sync(kFull, tc::next_block(&next_answer[n & 1]), 0) < 0) break;
+      }
+      if (!ok && lane == 0) failed = 1;
+    }
+  } else {
+    // ----------------------------------------------------------- softmax + epilogue
+    tc::regs_inc<kRegsSoftmax>();
+    const int t = (warp >> 2) - 1;           // tile of rows of this warp group
+    const int quad = warp & 3;               // TMEM lane quadrant this warp may touch
+    const int row = quad * 32 + lane;        // row inside the tile
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const uint32_t s_addr = lane_addr + kColS + t * 128;
+    const uint32_t o_addr = lane_addr + kColO + t * 128;
+    bool ok = true;
+    int seen = 0;   // score tiles of this tile of rows so far, over all items
+    int closed = 0; // items in which this tile of rows had work
+    for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
+      const Item w = item_of(index);
+      const int i0 = t ? w.i0[1] : w.i0[0], h0 = t ? w.h0[1] : w.h0[0], hi = t ? w.hi[1] : w.hi[0];
+      const int qi = i0 + (row & (R - 1)), h = h0 + (row >> p.rows_log2);
+      const int at = qi < w.q_len ? w.off + qi : -1;  // (below 0: sees nothing)
+      // every row of the tile sees all of a key tile that ends before the first row and begins in the last row's window
+      const int at_first = w.off + i0, at_last = w.off + min(i0 + R, w.q_len) - 1;
+      float m_used = -INFINITY;  // reference maximum (scaled, log2 domain)
+      float l = 0.f;             // running sum of exp2(s - m_used)
+      bool begun = false;
+      for (int x = 0; x < w.n_kv; ++x) {
+        if (!looks(w, t, x)) continue;
+        if (!__all_sync(kFull, mbar_wait(&s_full[t], seen & 1, &failed))) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        const int col0 = key_tile(w, x) * BN;
+        WindowMask mask;
+        mask.edge = col0 + BN - 1 > at_first || col0 <= at_last - p.window;
+        mask.lim = at - col0;
+        mask.from = col0 == 0 ? p.sinks : 0;
+        mask.low = at - p.window + 1 - col0;
+        softmax_tile<IS_BF16>(s_addr, o_addr, mask, !begun, p.scale_log2, m_used, l, &p_full[t], &p_rest[t]);
+        begun = true;
+        ++seen;
+      }
+      if (ok && hi > 0) {
+        ok = __all_sync(kFull, mbar_wait(&pv_done[t], closed & 1, &failed));  // the tile's last product
+        ++closed;
+      }
+      if (ok && h0 >= 0) {
+        tc::fence_after_sync();
+        if (at < 0) l = 0.f;  // (tiles that all other rows see whole are not masked)
+        const float inv = (l > 0.f) ? 1.f / l : (l == 0.f ? 0.f : l);  // (l may be NaN)
+        const bool live = qi < p.Sq && h < (w.hk + 1) * p.share;
+        unsigned char* orow = reinterpret_cast<unsigned char*>(p.o) +
+                              2 * ((long long)w.b * p.o_stride_b + (long long)h * p.o_stride_h +
+                                   (long long)qi * p.o_stride_s);
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          if (hi > 0) {
+            tc::tmem_ld32(o_addr + c * 32, o);
+            tc::tmem_wait_ld();
+          }
+          if (l == 0.f) {  // nothing was seen
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (live) tc::store_row32<IS_BF16>(orow + c * 64, o, inv, p.wide != 0);
+        }
+        if (live && p.lse != nullptr) {
+          const float lse = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994530942f;  // (l may be NaN)
+          p.lse[((long long)w.b * p.H + h) * p.Sq + qi] = lse;
+        }
+      }
+      // (the next item's scores may be written meanwhile, but its first product waits for this
+      // warp's probabilities, which come after the reads of O above)
+      tc::fence_before_sync();
+      index = take_next(n, ok);
+    }
+    if (!ok && lane == 0) failed = 1;
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (failed) {  // (uniform: nobody writes it any more)
+    // a role gave up: what the others have under way has to end before the block does
+    if (threadIdx.x == 0) {
+      tc::await_copies<1>(&q_full, q_loads);
+      tc::await_copies<kStages>(k_full, k_loads);
+      if (raw_pending) mbar_wait(&v_raw, (raw_loads - 1) & 1);
+      tc::await_copies<kStages>(v_full, v_loads);
+    }
+    if (warp == 1) tc::await_products(&drained);
+    if (warp == 2 && lane == 0) tc::await_copies<2>(next_full, asked);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && failed && p.status != nullptr) atomicExch(p.status, 1);
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace
+
+namespace ixb_host {
+
+int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
+                   float* lse, int32_t* status, cudaStream_t stream) {
+  WinParams p;
+  p.rows_log2 = 3;
+  while (p.rows_log2 < 7 && (1 << p.rows_log2) < a.Sq) ++p.rows_log2;
+  CUtensorMap mq, mk, mv;
+  if (int st = make_fa_map(&mq, q.ptr, a.is_bf16, a.B, a.H, a.Sq, q.strides[0], q.strides[1], q.strides[2], 1 << p.rows_log2)) return st;
+  if (int st = make_fa_map(&mk, k.ptr, a.is_bf16, a.B, a.HK, a.Sk, k.strides[0], k.strides[1], k.strides[2])) return st;
+  if (int st = make_fa_map(&mv, v.ptr, a.is_bf16, a.B, a.HK, a.Sk, v.strides[0], v.strides[1], v.strides[2])) return st;
+  p.o = const_cast<void*>(o.ptr);
+  p.lse = lse;
+  p.status = status;
+  p.q_lengths = a.q_lengths;
+  p.kv_lengths = a.kv_lengths;
+  p.o_stride_b = o.strides[0];
+  p.o_stride_h = o.strides[1];
+  p.o_stride_s = o.strides[2];
+  p.B = a.B, p.H = a.H, p.HK = a.HK, p.share = a.H / a.HK, p.Sq = a.Sq, p.Sk = a.Sk;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.window = a.window, p.sinks = a.sinks;
+  const int heads = BM >> p.rows_log2;  // query heads in a tile
+  const long long tiles = (long long)((a.Sq + BM - 1) / BM) * ((p.share + heads - 1) / heads);
+  const long long items = (tiles + NQ - 1) / NQ * a.B * a.HK;
+  if (items > 0x7fffffffLL) return IXB_ERR_SHAPE;
+  p.tiles = (int)tiles;
+  p.wide = rows_aligned32(o.ptr, o.strides) ? 1 : 0;
+  auto kern = a.is_bf16 ? fa_window_fwd_kernel<true> : fa_window_fwd_kernel<false>;
+  // the shared-memory opt-in is a property of (kernel, device): set once per device
+  static std::atomic<bool> configured[2][64];
+  int devid = 0;
+  cudaGetDevice(&devid);
+  std::atomic<bool>& done = configured[a.is_bf16][devid & 63];
+  if (!done.load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaFuncAttributes at;  // (as in fa_fwd.cu: the softmax warps wait for registers the block has to own)
+    e = cudaFuncGetAttributes(&at, kern);
+    if (e != cudaSuccess) return cuda_status(e);
+    if (at.numRegs != kRegsLaunch) return IXB_ERR_UNSUPPORTED;
+    done.store(true, std::memory_order_release);
+  }
+  kern<<<(unsigned)items, kThreads, kSmemBytes, stream>>>(mq, mk, mv, p);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace ixb_host

@@ -27,12 +27,29 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi, bool is_bf16) 
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Hides keys behind `lim` (relative to the tile) from a row, where the tile is an `edge`.
+struct CausalMask {
+  bool edge;
+  int lim;
+  __device__ __forceinline__ void apply(uint32_t (&raw)[BN]) const {
+    if (edge) {
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        if (__all_sync(kFull, lim >= c * 32 + 31)) continue;  // (what every row of the warp sees stays)
+#pragma unroll
+        for (int e = c * 32; e < c * 32 + 32; ++e)
+          if (e > lim) raw[e] = 0xff800000u;  // -inf
+      }
+    }
+  }
+};
+
 // Scores of this thread's row (tensor memory at s_addr) to probabilities relative to the running reference
 // maximum m_used, written over them as 16-bit pairs and handed over in two parts (p_full after kSplit keys,
-// p_rest); l grows by their sum.  `edge`: keys behind `lim` (relative to the tile) are hidden from this
-// row.  `first`: the row's accumulator at o_addr holds nothing yet.
-template <bool IS_BF16>
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, bool edge, int lim, bool first, float scale_log2,
+// p_rest); l grows by their sum.  `mask` hides keys of the tile from this row.  `first`: the row's accumulator at
+// o_addr holds nothing yet.
+template <bool IS_BF16, class Mask>
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const Mask& mask, bool first, float scale_log2,
                                              float& m_used, float& l, uint64_t* p_full, uint64_t* p_rest) {
   // the row of scores stays in registers: one trip through tensor memory per tile
   uint32_t raw[BN];
@@ -40,15 +57,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, b
   for (int c = 0; c < BN / 32; ++c)
     tc::tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[c * 32]));
   tc::tmem_wait_ld();
-  if (edge) {
-#pragma unroll
-    for (int c = 0; c < BN / 32; ++c) {
-      if (__all_sync(kFull, lim >= c * 32 + 31)) continue;  // (what every row of the warp sees stays)
-#pragma unroll
-      for (int e = c * 32; e < c * 32 + 32; ++e)
-        if (e > lim) raw[e] = 0xff800000u;  // -inf
-    }
-  }
+  mask.apply(raw);
   // four independent chains: one chain of 64 dependent max3 would cost its latency 64 times
   float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
