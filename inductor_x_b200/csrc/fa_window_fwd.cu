@@ -480,3 +480,19 @@ int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& 
 }
 
 }  // namespace ixb_host
+
+extern "C" size_t ixb_window_attention_scratch_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+
+extern "C" int ixb_window_attention(int dtype, const void* q, const void* k, const void* v, void* o, float* lse, void*,
+                                    size_t, int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk, int32_t D,
+                                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                    const int64_t* o_strides, const int32_t* q_lengths, const int32_t* kv_lengths, float scale,
+                                    int32_t window, int32_t sinks, int32_t* status, ixb_stream stream) {
+  if (int st = ixb_host::check_window_sizes(dtype, B, H, HK, Sq, Sk, D, scale, window, sinks)) return st;
+  if (B == 0 || H == 0 || Sq == 0) return IXB_OK;
+  if (Sk == 0) return IXB_ERR_SHAPE;
+  const ixb_host::WindowView views[] = {{q, q_strides}, {k, k_strides}, {v, v_strides}, {o, o_strides}};
+  if (int st = ixb_host::check_window_views(views, 4)) return st;
+  const ixb_host::WindowShape a{dtype == IXB_BF16, B, H, HK, Sq, Sk, q_lengths, kv_lengths, scale, window < Sk ? window : Sk, sinks};
+  return ixb_host::window_prefill(a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
+}
