@@ -1,4 +1,7 @@
 // Rotary positions with several axes: pair i of a head is turned by the angle position[axis(i)] * frequency(i).
+// Sines and cosines are formed once a token, for all heads of q and k; a thread keeps those of its pairs while it walks the
+// heads, and asks for its first values before it forms them.
+// Bound: memory, every value read and written once.
 #include <cmath>
 #include "host.h"
 #include "ixb/common.cuh"
@@ -24,19 +27,86 @@ struct RotaryParams {
   unsigned char axis[kMaxPairs];
 };
 
-// a block a token
-template <class T> __global__ void rotary_kernel(const __grid_constant__ RotaryParams p) {
+// The turn of pair i for token (b, s): in whole turns and 64 bits until the fraction is known - 32 bits hold nothing of a far
+// position's.
+__device__ __forceinline__ float2 turn_of(const RotaryParams& p, int i, int b, int s) {
+  const long long at = p.axis[i] * p.pos_sa + b * p.pos_sb + s * p.pos_ss;
+  const double pos = p.wide ? (double)static_cast<const long long*>(p.positions)[at] : (double)static_cast<const int*>(p.positions)[at];
+  const double t = pos * p.turns[i];
+  float sn, c;
+  sincospif(2.f * (float)(t - rint(t)), &sn, &c);
+  return make_float2(c, p.inverse ? -sn : sn);
+}
+
+// Vectors: a part is kVec pairs of a head, two vectors of it, or one of the vectors behind the pairs.  A block takes `tokens`
+// tokens and all heads; a thread is a part of a token and walks heads, `threads / (parts * tokens)` apart.
+template <class T> __global__ void __launch_bounds__(256) rotary_vector_kernel(const __grid_constant__ RotaryParams p, int parts, int tokens, int slots,
+                                                                                int heads_first) {
+  constexpr int kVec = Elem<T>::kVec;
+  extern __shared__ float2 cs[];  // [tokens][pairs]
+  const int part = threadIdx.x % parts, place = threadIdx.x / parts;
+  const int token = heads_first ? place / slots : place % tokens, slot = heads_first ? place % slots : place / tokens;
+  const long long first = (long long)blockIdx.x * tokens, all = (long long)p.B * p.S;
+  const bool live = place < slots * tokens && first + token < all;
+  const int b = (int)((first + token) / p.S), s = (int)((first + token) % p.S);
+  const int turned = p.pairs / kVec;
+  const bool copies = part >= turned;
+  const int lo = copies ? 2 * p.pairs + (part - turned) * kVec : p.neighbours ? 2 * kVec * part : kVec * part;
+  const int hi = copies ? lo : p.neighbours ? lo + kVec : lo + p.pairs;
+  uint4 va, vb;
+  auto fetch = [&](int which, int h) {
+    const Operand& x = p.x[which];
+    const T* in = static_cast<const T*>(x.in) + b * x.in_sb + s * x.in_ss + h * x.in_sh;
+    va = ldg_stream(in + lo);
+    if (!copies) vb = ldg_stream(in + hi);
+  };
+  int which = p.x[0].heads > slot ? 0 : 1, h = slot;
+  bool more = live && h < p.x[which].heads;
+  if (more) fetch(which, h);
+  for (int u = threadIdx.x; u < tokens * p.pairs; u += blockDim.x) {
+    const int k = u / p.pairs;
+    if (first + k < all) cs[u] = turn_of(p, u - k * p.pairs, (int)((first + k) / p.S), (int)((first + k) % p.S));
+  }
+  __syncthreads();
+  float2 turn[kVec];
+  if (live && !copies) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) turn[e] = cs[token * p.pairs + part * kVec + e];
+  }
+  while (more) {
+    const Operand& x = p.x[which];
+    T* out = static_cast<T*>(x.out) + b * x.out_sb + s * x.out_ss + h * x.out_sh;
+    const uint4 a = va, c = vb;
+    h += slots;
+    if (which == 0 && h >= p.x[0].heads) {
+      which = 1;
+      h = slot;
+    }
+    more = h < p.x[which].heads;
+    if (more) fetch(which, h);
+    if (copies) {
+      *reinterpret_cast<uint4*>(out + lo) = a;
+      continue;
+    }
+    float f[2 * kVec], g[2 * kVec];
+    unpack<T>(a, f);
+    unpack<T>(c, f + kVec);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const int i = p.neighbours ? 2 * e : e, j = p.neighbours ? 2 * e + 1 : e + kVec;
+      g[i] = f[i] * turn[e].x - f[j] * turn[e].y;
+      g[j] = f[i] * turn[e].y + f[j] * turn[e].x;
+    }
+    *reinterpret_cast<uint4*>(out + lo) = pack<T>(g);
+    *reinterpret_cast<uint4*>(out + hi) = pack<T>(g + kVec);
+  }
+}
+
+// Heads that are no whole vectors, or off a boundary: a block a token, pair by pair.
+template <class T> __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ float2 cs[kMaxPairs];
   const int b = blockIdx.x / p.S, s = blockIdx.x % p.S;
-  for (int i = threadIdx.x; i < p.pairs; i += blockDim.x) {
-    const long long at = p.axis[i] * p.pos_sa + b * p.pos_sb + s * p.pos_ss;
-    const double pos = p.wide ? (double)static_cast<const long long*>(p.positions)[at] : (double)static_cast<const int*>(p.positions)[at];
-    // in whole turns and 64 bits until the fraction is known: 32 bits hold nothing of a far position's
-    const double t = pos * p.turns[i];
-    float sn, c;
-    sincospif(2.f * (float)(t - rint(t)), &sn, &c);
-    cs[i] = make_float2(c, p.inverse ? -sn : sn);
-  }
+  for (int i = threadIdx.x; i < p.pairs; i += blockDim.x) cs[i] = turn_of(p, i, b, s);
   __syncthreads();
   for (int which = 0; which < 2; ++which) {
     const Operand& x = p.x[which];
@@ -54,6 +124,34 @@ template <class T> __global__ void rotary_kernel(const __grid_constant__ RotaryP
       out[h * x.out_sh + e] = in[h * x.in_sh + e];
     }
   }
+}
+
+template <class T> int run(const RotaryParams& p, cudaStream_t stream) {
+  constexpr int kVec = Elem<T>::kVec;
+  bool vectors = p.pairs % kVec == 0 && p.D % kVec == 0;
+  for (const Operand& x : p.x)
+    vectors = vectors && (x.heads == 0 || (ixb_host::aligned16(x.in) && ixb_host::aligned16(x.out) &&
+                                           ((x.in_sb | x.in_sh | x.in_ss | x.out_sb | x.out_sh | x.out_ss) & (kVec - 1)) == 0));
+  const long long all = (long long)p.B * p.S;
+  if (!vectors) {
+    rotary_kernel<T><<<(unsigned)all, 256, 0, stream>>>(p);
+    return ixb_host::cuda_status(cudaGetLastError());
+  }
+  const int parts = p.pairs / kVec + (p.D - 2 * p.pairs) / kVec;
+  const int heads = p.x[0].heads > p.x[1].heads ? p.x[0].heads : p.x[1].heads;
+  // neighbouring threads take neighbouring memory: the heads of a token where they follow one another, else tokens of a head
+  const Operand& x = p.x[p.x[0].heads > 0 ? 0 : 1];
+  const int heads_first = x.in_sh <= x.in_ss || p.S == 1;
+  const int places = 256 / parts;
+  int slots = heads_first ? (heads < places ? heads : places) : 1, tokens = places / slots;
+  if (!heads_first) {
+    if (tokens > 16) tokens = 16;
+    slots = places / tokens < heads ? places / tokens : heads;
+  }
+  if (tokens > 16) tokens = 16;
+  rotary_vector_kernel<T><<<(unsigned)((all + tokens - 1) / tokens), 256, tokens * p.pairs * sizeof(float2), stream>>>(p, parts, tokens, slots,
+                                                                                                                   heads_first);
+  return ixb_host::cuda_status(cudaGetLastError());
 }
 
 }  // namespace
@@ -91,9 +189,7 @@ extern "C" int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int
   p.pos_sa = position_strides[0], p.pos_sb = position_strides[1], p.pos_ss = position_strides[2];
   p.wide = position_dtype == IXB_I64;
   p.B = B, p.S = S, p.D = D, p.neighbours = neighbours != 0, p.inverse = inverse != 0;
-  const unsigned grid = (unsigned)((long long)B * S);
-  if (dtype == IXB_BF16) rotary_kernel<bf16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  else if (dtype == IXB_F16) rotary_kernel<f16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  else rotary_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  return ixb_host::cuda_status(cudaGetLastError());
+  if (dtype == IXB_BF16) return run<bf16>(p, (cudaStream_t)stream);
+  if (dtype == IXB_F16) return run<f16>(p, (cudaStream_t)stream);
+  return run<float>(p, (cudaStream_t)stream);
 }
