@@ -10,6 +10,7 @@ namespace {
 
 using namespace ixb;
 constexpr int kMaxPairs = 128;
+constexpr int kMaxTurns = 2048;  // a block's, 16 KB
 
 struct Operand {
   const void* in;
@@ -23,82 +24,123 @@ struct RotaryParams {
   long long pos_sa, pos_sb, pos_ss;
   int wide;        // positions of 64 bits
   int B, S, D, pairs, neighbours, inverse;
-  double turns[kMaxPairs];          // whole turns a position
+  unsigned long long turns[kMaxPairs];  // 2^-64 of a turn a position
   unsigned char axis[kMaxPairs];
 };
 
-// The turn of pair i for token (b, s): in whole turns and 64 bits until the fraction is known - 32 bits hold nothing of a far
-// position's.
+// The turn of pair i for token (b, s).  The product of a position and a frequency in 2^-64 of a turn wraps around at whole turns
+// by itself, so that a far position keeps its fraction of one; its upper half is that fraction to 2^-32.
+// The parameters are read by their generic address: lanes that read different ones as constants take turns.
 __device__ __forceinline__ float2 turn_of(const RotaryParams& p, int i, int b, int s) {
-  const long long at = p.axis[i] * p.pos_sa + b * p.pos_sb + s * p.pos_ss;
-  const double pos = p.wide ? (double)static_cast<const long long*>(p.positions)[at] : (double)static_cast<const int*>(p.positions)[at];
-  const double t = pos * p.turns[i];
+  unsigned long long turns;
+  unsigned axis;
+  asm("ld.u64 %0, [%1];" : "=l"(turns) : "l"(&p.turns[i]));
+  asm("ld.u8 %0, [%1];" : "=r"(axis) : "l"(&p.axis[i]));
+  const long long at = axis * p.pos_sa + b * p.pos_sb + s * p.pos_ss;
+  const long long pos = p.wide ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
+  const int fraction = (int)(((unsigned long long)pos * turns) >> 32);  // in [-1/2, 1/2) of a turn
   float sn, c;
-  sincospif(2.f * (float)(t - rint(t)), &sn, &c);
+  sincospif((float)fraction * 0x1p-31f, &sn, &c);
   return make_float2(c, p.inverse ? -sn : sn);
 }
 
+// The pairs of two vectors: (low[e], high[e]), or the neighbours of low and then of high.
+template <class T, bool NEIGHBOURS, int N> __device__ __forceinline__ void turn_pairs(uint4& low, uint4& high, const float2 (&turn)[N]) {
+  float f[N], g[N];
+  unpack<T>(low, f);
+  unpack<T>(high, g);
+  if constexpr (NEIGHBOURS) {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      const float a = f[2 * e], c = f[2 * e + 1], d = g[2 * e], h = g[2 * e + 1];
+      f[2 * e] = a * turn[e].x - c * turn[e].y;
+      f[2 * e + 1] = a * turn[e].y + c * turn[e].x;
+      g[2 * e] = d * turn[N / 2 + e].x - h * turn[N / 2 + e].y;
+      g[2 * e + 1] = d * turn[N / 2 + e].y + h * turn[N / 2 + e].x;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float a = f[e], c = g[e];
+      f[e] = a * turn[e].x - c * turn[e].y;
+      g[e] = a * turn[e].y + c * turn[e].x;
+    }
+  }
+  low = pack<T>(f);
+  high = pack<T>(g);
+}
+
 // Vectors: a part is kVec pairs of a head, two vectors of it, or one of the vectors behind the pairs.  A block takes `tokens`
-// tokens and all heads; a thread is a part of a token and walks heads, `threads / (parts * tokens)` apart.
-template <class T> __global__ void __launch_bounds__(256) rotary_vector_kernel(const __grid_constant__ RotaryParams p, int parts, int tokens, int slots,
-                                                                                int heads_first) {
+// tokens at a time and all heads of them, q's and then k's; a thread is a part of a token and walks heads `slots`
+// apart, kAhead of them in flight.
+// 2 x 8192 tokens of 32 + 8 heads, there and back: 128 threads and 5 heads in flight 109 us (94 % of a copy's rate), the same on
+// 256 threads 124, 4 heads in flight on those 128, 3 or 2 190; blocks that go on to further tokens 120 - 142, with the next
+// heads asked for as each is done 143 - 173 (loads and stores in turn cost more than waiting).
+constexpr int kAhead = 5, kThreads = 128;
+template <class T, bool NEIGHBOURS>
+__global__ void __launch_bounds__(kThreads, 5) rotary_vector_kernel(const __grid_constant__ RotaryParams p, int parts, int tokens, int slots, int heads_first) {
   constexpr int kVec = Elem<T>::kVec;
   extern __shared__ float2 cs[];  // [tokens][pairs]
   const int part = threadIdx.x % parts, place = threadIdx.x / parts;
   const int token = heads_first ? place / slots : place % tokens, slot = heads_first ? place % slots : place / tokens;
-  const long long first = (long long)blockIdx.x * tokens, all = (long long)p.B * p.S;
-  const bool live = place < slots * tokens && first + token < all;
-  const int b = (int)((first + token) / p.S), s = (int)((first + token) % p.S);
-  const int turned = p.pairs / kVec;
+  const int all = p.B * p.S, heads = p.x[0].heads + p.x[1].heads, turned = p.pairs / kVec;
   const bool copies = part >= turned;
-  const int lo = copies ? 2 * p.pairs + (part - turned) * kVec : p.neighbours ? 2 * kVec * part : kVec * part;
-  const int hi = copies ? lo : p.neighbours ? lo + kVec : lo + p.pairs;
-  uint4 va, vb;
-  auto fetch = [&](int which, int h) {
-    const Operand& x = p.x[which];
-    const T* in = static_cast<const T*>(x.in) + b * x.in_sb + s * x.in_ss + h * x.in_sh;
-    va = ldg_stream(in + lo);
-    if (!copies) vb = ldg_stream(in + hi);
+  const int lo = copies ? 2 * p.pairs + (part - turned) * kVec : NEIGHBOURS ? 2 * kVec * part : kVec * part;
+  const int hi = copies ? lo : NEIGHBOURS ? lo + kVec : lo + p.pairs;
+  const int first = blockIdx.x * tokens;
+  const bool live = place < slots * tokens && first + token < all;
+  const int b = (first + token) / p.S, s = (first + token) - b * p.S;
+  const T* in[2];
+  T* out[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    in[w] = static_cast<const T*>(p.x[w].in) + b * p.x[w].in_sb + s * p.x[w].in_ss;
+    out[w] = static_cast<T*>(p.x[w].out) + b * p.x[w].out_sb + s * p.x[w].out_ss;
+  }
+  uint4 va[kAhead], vb[kAhead];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = h0 + i * slots;
+      if (!live || h >= heads) continue;
+      const T* from = h < p.x[0].heads ? in[0] + h * p.x[0].in_sh : in[1] + (h - p.x[0].heads) * p.x[1].in_sh;
+      va[i] = ldg_stream(from + lo);
+      if (!copies) vb[i] = ldg_stream(from + hi);
+    }
   };
-  int which = p.x[0].heads > slot ? 0 : 1, h = slot;
-  bool more = live && h < p.x[which].heads;
-  if (more) fetch(which, h);
-  for (int u = threadIdx.x; u < tokens * p.pairs; u += blockDim.x) {
-    const int k = u / p.pairs;
-    if (first + k < all) cs[u] = turn_of(p, u - k * p.pairs, (int)((first + k) / p.S), (int)((first + k) % p.S));
+  fetch(slot);
+  const int b0 = first / p.S, s0 = first - b0 * p.S;
+  const unsigned per_pair = (1u << 20) / p.pairs + 1;  // (u / pairs is exact so below kMaxTurns)
+  for (int u = threadIdx.x; u < tokens * p.pairs; u += kThreads) {
+    const int k = (int)((u * per_pair) >> 20);
+    int tb = b0, ts = s0 + k;
+    while (ts >= p.S) {
+      ts -= p.S;
+      ++tb;
+    }
+    if (first + k < all) cs[u] = turn_of(p, u - k * p.pairs, tb, ts);
   }
   __syncthreads();
+  if (!live) return;
   float2 turn[kVec];
-  if (live && !copies) {
+  if (!copies) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) turn[e] = cs[token * p.pairs + part * kVec + e];
   }
-  while (more) {
-    const Operand& x = p.x[which];
-    T* out = static_cast<T*>(x.out) + b * x.out_sb + s * x.out_ss + h * x.out_sh;
-    const uint4 a = va, c = vb;
-    h += slots;
-    if (which == 0 && h >= p.x[0].heads) {
-      which = 1;
-      h = slot;
-    }
-    more = h < p.x[which].heads;
-    if (more) fetch(which, h);
-    if (copies) {
-      *reinterpret_cast<uint4*>(out + lo) = a;
-      continue;
-    }
-    float f[2 * kVec], g[2 * kVec];
-    unpack<T>(a, f);
-    unpack<T>(c, f + kVec);
+  for (int h0 = slot; h0 < heads; h0 += kAhead * slots) {
+    if (h0 > slot) fetch(h0);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const int i = p.neighbours ? 2 * e : e, j = p.neighbours ? 2 * e + 1 : e + kVec;
-      g[i] = f[i] * turn[e].x - f[j] * turn[e].y;
-      g[j] = f[i] * turn[e].y + f[j] * turn[e].x;
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = h0 + i * slots;
+      if (h >= heads) break;
+      T* to = h < p.x[0].heads ? out[0] + h * p.x[0].out_sh : out[1] + (h - p.x[0].heads) * p.x[1].out_sh;
+      uint4 low = va[i], high = vb[i];
+      if (!copies) {
+        turn_pairs<T, NEIGHBOURS>(low, high, turn);
+        *reinterpret_cast<uint4*>(to + hi) = high;
+      }
+      *reinterpret_cast<uint4*>(to + lo) = low;
     }
-    *reinterpret_cast<uint4*>(out + lo) = pack<T>(g);
-    *reinterpret_cast<uint4*>(out + hi) = pack<T>(g + kVec);
   }
 }
 
@@ -128,7 +170,8 @@ template <class T> __global__ void __launch_bounds__(256) rotary_kernel(const __
 
 template <class T> int run(const RotaryParams& p, cudaStream_t stream) {
   constexpr int kVec = Elem<T>::kVec;
-  bool vectors = p.pairs % kVec == 0 && p.D % kVec == 0;
+  const int parts = p.pairs / kVec + (p.D - 2 * p.pairs) / kVec;
+  bool vectors = p.pairs % kVec == 0 && p.D % kVec == 0 && parts <= 32;
   for (const Operand& x : p.x)
     vectors = vectors && (x.heads == 0 || (ixb_host::aligned16(x.in) && ixb_host::aligned16(x.out) &&
                                            ((x.in_sb | x.in_sh | x.in_ss | x.out_sb | x.out_sh | x.out_ss) & (kVec - 1)) == 0));
@@ -137,20 +180,22 @@ template <class T> int run(const RotaryParams& p, cudaStream_t stream) {
     rotary_kernel<T><<<(unsigned)all, 256, 0, stream>>>(p);
     return ixb_host::cuda_status(cudaGetLastError());
   }
-  const int parts = p.pairs / kVec + (p.D - 2 * p.pairs) / kVec;
-  const int heads = p.x[0].heads > p.x[1].heads ? p.x[0].heads : p.x[1].heads;
+  const ixb_devinfo* dev = ixb_host::current_device();
+  if (dev == nullptr) return IXB_ERR_CUDA;
+  const int heads = p.x[0].heads + p.x[1].heads;
   // neighbouring threads take neighbouring memory: the heads of a token where they follow one another, else tokens of a head
   const Operand& x = p.x[p.x[0].heads > 0 ? 0 : 1];
-  const int heads_first = x.in_sh <= x.in_ss || p.S == 1;
-  const int places = 256 / parts;
-  int slots = heads_first ? (heads < places ? heads : places) : 1, tokens = places / slots;
-  if (!heads_first) {
-    if (tokens > 16) tokens = 16;
-    slots = places / tokens < heads ? places / tokens : heads;
-  }
-  if (tokens > 16) tokens = 16;
-  rotary_vector_kernel<T><<<(unsigned)((all + tokens - 1) / tokens), 256, tokens * p.pairs * sizeof(float2), stream>>>(p, parts, tokens, slots,
-                                                                                                                   heads_first);
+  const int heads_first = x.in_sh <= x.in_ss || p.S == 1, places = kThreads / parts;
+  // about kAhead heads a thread, fewer where that leaves SMs without a block
+  int tokens = places * kAhead / heads;
+  if (tokens * p.pairs > kMaxTurns) tokens = kMaxTurns / p.pairs;
+  if (!heads_first && tokens < 4) tokens = 4;
+  while (tokens > 1 && (all + tokens - 1) / tokens < 2 * dev->sm_count) tokens /= 2;
+  if (tokens < 1) tokens = 1;
+  if (tokens > places) tokens = places;
+  const int slots = places / tokens < heads ? places / tokens : heads;
+  auto kern = p.neighbours ? rotary_vector_kernel<T, true> : rotary_vector_kernel<T, false>;
+  kern<<<(unsigned)((all + tokens - 1) / tokens), kThreads, tokens * p.pairs * sizeof(float2), stream>>>(p, parts, tokens, slots, heads_first);
   return ixb_host::cuda_status(cudaGetLastError());
 }
 
@@ -170,13 +215,15 @@ extern "C" int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int
     if (sections[a] < 0) return IXB_ERR_ARG;
     if (axes > kMaxPairs || sections[a] > kMaxPairs - p.pairs) return IXB_ERR_SHAPE;
     for (int j = 0; j < sections[a]; ++j, ++p.pairs) {
-      p.turns[p.pairs] = frequencies[p.pairs] * 0.15915494309189533577;  // 1 / (2 pi)
+      const long double turns = frequencies[p.pairs] / 6.283185307179586476925286766559L;
+      if (!std::isfinite(frequencies[p.pairs])) return IXB_ERR_ARG;
+      p.turns[p.pairs] = (unsigned long long)std::ldexp(turns - std::floor(turns), 64);
       p.axis[p.pairs] = (unsigned char)a;
     }
   }
   if (2 * p.pairs > D) return IXB_ERR_SHAPE;
   if (B == 0 || S == 0 || D == 0 || heads + (long long)k_heads == 0) return IXB_OK;
-  if ((long long)B * S > 0x7fffffffLL) return IXB_ERR_SHAPE;
+  if ((long long)B * S > (1 << 30)) return IXB_ERR_SHAPE;
   if ((heads && (!q || !q_out || !q_strides || !q_out_strides)) || (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) ||
       !positions || !position_strides)
     return IXB_ERR_ARG;
