@@ -215,9 +215,10 @@ extern "C" int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int
     if (sections[a] < 0) return IXB_ERR_ARG;
     if (axes > kMaxPairs || sections[a] > kMaxPairs - p.pairs) return IXB_ERR_SHAPE;
     for (int j = 0; j < sections[a]; ++j, ++p.pairs) {
-      const long double turns = frequencies[p.pairs] / 6.283185307179586476925286766559L;
       if (!std::isfinite(frequencies[p.pairs])) return IXB_ERR_ARG;
-      p.turns[p.pairs] = (unsigned long long)std::ldexp(turns - std::floor(turns), 64);
+      const long double turns = std::fabs(frequencies[p.pairs]) / 6.283185307179586476925286766559L;
+      const unsigned long long part = (unsigned long long)std::ldexp(turns - std::floor(turns), 64);
+      p.turns[p.pairs] = frequencies[p.pairs] < 0 ? 0 - part : part;
       p.axis[p.pairs] = (unsigned char)a;
     }
   }

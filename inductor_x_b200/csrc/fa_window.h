@@ -40,5 +40,9 @@ inline int check_window_views(const WindowView* views, int n) {
 // fa_window_fwd.cu
 int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
                    float* lse, int32_t* status, cudaStream_t stream);
+// fa_window_decode.cu: whether it takes a call, and the call
+bool window_decodes(const WindowShape& a);
+int window_decode(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
+                  float* lse, int32_t* status, cudaStream_t stream);
 
 }  // namespace ixb_host

@@ -1,0 +1,436 @@
+// Windowed attention of a few queries over a long cache: the decoding step (the meaning of the arguments: fa_window.h).
+// All that a key head's queries need is read once: the rows of a block are those of every query head that shares the key
+// head (R = queries x sharing heads, in groups of 16 x MT), and the keys are the first tokens that lie in front of the
+// window and the window itself, cut into tiles of 16.  The tiles are shared over the kWarps warps of 1, 2, 4 or 8 blocks of a
+// cluster.  A warp keeps its own running maximum, sum and accumulators and has its own ring of copies: nothing waits
+// for another warp before the end, when the warps of a block and then the blocks of the cluster add up, row by row
+// through distributed shared memory: one launch, no scratch, the same bits every time.
+//
+// Bound: memory.  A key costs 512 bytes and, per row, 512 multiplications, so that warp-wide 16 x 8 x 16 products are
+// enough.  Both operands of both products come out of shared memory as whole 16-byte pieces: the order of the reduced
+// dimensions of S = Q K^T is free, so a lane's piece of 8 dimensions is taken for four of its pairs; the columns of
+// O = P V are free too, so a lane pairs up its pieces of two keys element by element.
+#include <atomic>
+#include "fa_window.h"
+#include "ixb/tcgen05.cuh"
+
+namespace {
+
+using namespace ixb;
+
+constexpr int HD = 128, kTile = 16, kWarps = 4, kThreads = kWarps * 32, kStages = 3;
+constexpr int kBoxBytes = kTile * 128;        // 16 keys of 64 dimensions
+constexpr int kStageBytes = 4 * kBoxBytes;    // K and V
+constexpr int kPitch = HD + 4;                // floats: of a row of partial sums
+constexpr size_t kSmemBytes = (size_t)kWarps * kStages * kStageBytes + 1024;
+
+struct DecodeParams {
+  const unsigned char* q;
+  unsigned char* o;
+  float* lse;     // [B, H, Sq], may be null
+  int* status;    // may be null
+  const int *q_lengths, *kv_lengths;
+  long long q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;  // elements
+  int H, HK, share, Sq, Sk, rows, groups;        // rows = share * Sq, in `groups` of 16 * MT
+  float scale_log2;
+  int window, sinks;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(const void* local_smem, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local_smem)), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// d += a b: 16 rows x 16, 16 x 8
+template <bool IS_BF16> __device__ __forceinline__ void product(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (IS_BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// piece `chunk` (16 bytes of 8 dimensions) of key `key` in a box of 128-byte rows that the copy engine has swizzled
+__device__ __forceinline__ uint4 piece(const unsigned char* box, int key, int chunk) {
+  return *reinterpret_cast<const uint4*>(box + key * 128 + ((chunk ^ (key & 7)) << 4));
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+template <bool IS_BF16, int MT, int CLUSTER>
+__global__ void __launch_bounds__(kThreads, 2)
+    window_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeParams p) {
+  constexpr int kRows = 16 * MT;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t full[kWarps][kStages];
+  __shared__ float m_part[kWarps][kRows], l_part[kWarps][kRows], m_block[kRows], l_block[kRows];
+  __shared__ volatile int failed;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
+  const int rank = CLUSTER > 1 ? (int)cluster_rank() : 0;
+  const int item = (int)blockIdx.x / CLUSTER, group = item % p.groups, bh = item / p.groups, b = bh / p.HK, hk = bh - b * p.HK;
+  const int row0 = group * kRows;
+  const int q_len = p.q_lengths != nullptr ? min(max(__ldg(p.q_lengths + b), 0), p.Sq) : p.Sq;
+  const int kv_len = p.kv_lengths != nullptr ? min(max(__ldg(p.kv_lengths + b), 0), p.Sk) : p.Sk;
+  const int off = kv_len - q_len;  // query i stands at position off + i
+  const bool any = q_len > 0 && kv_len > 0;
+  // keys [0, front) and [low, kv_len) are seen by some query
+  const int low = any ? max(max(off, 0) - p.window + 1, 0) : 0, front = any ? min(p.sinks, low) : 0;
+  const int front_tiles = (front + kTile - 1) / kTile, tiles = any ? front_tiles + (kv_len - low + kTile - 1) / kTile : 0;
+  auto first_key = [&](int t) { return t < front_tiles ? t * kTile : low + (t - front_tiles) * kTile; };
+  const int worker = rank * kWarps + warp;
+  constexpr int kWorkers = CLUSTER * kWarps;
+  const int mine = tiles > worker ? (tiles - worker + kWorkers - 1) / kWorkers : 0;
+
+  if (threadIdx.x == 0) failed = 0;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
+    mbar_init_fence();
+  }
+  __syncthreads();
+  unsigned char* ring = smem + warp * kStages * kStageBytes;
+  auto ask = [&](int i) {  // tile i of this warp (one lane)
+    unsigned char* dst = ring + i % kStages * kStageBytes;
+    uint64_t* bar = &full[warp][i % kStages];
+    const int key = first_key(worker + i * kWorkers);
+    mbar_arrive_expect_tx(bar, kStageBytes);
+    tc::tma_load_4d(dst, &map_k, bar, 0, key, hk, b);
+    tc::tma_load_4d(dst + kBoxBytes, &map_k, bar, 64, key, hk, b);
+    tc::tma_load_4d(dst + 2 * kBoxBytes, &map_v, bar, 0, key, hk, b);
+    tc::tma_load_4d(dst + 3 * kBoxBytes, &map_v, bar, 64, key, hk, b);
+  };
+  if (lane == 0)
+    for (int i = 0; i < kStages && i < mine; ++i) ask(i);
+
+  // Q: rows n and n + 8 of each 16.  Piece 2c + odd of a half of 64 dimensions is two of the lane's steps of 16.
+  uint32_t qf[MT][8][4];
+  int at[MT][2];  // position of the row's query (below 0: sees nothing)
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = row0 + t * 16 + half * 8 + n, g = r / p.Sq, i = r - g * p.Sq;
+      const bool live = r < p.rows && i < q_len;
+      at[t][half] = live ? off + i : -1;
+      const unsigned char* src = p.q + 2 * (b * p.q_sb + (hk * p.share + g) * p.q_sh + i * p.q_ss);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 v = live ? ldg_keep(src + 2 * (k / 2 * 64 + (2 * c + k % 2) * 8)) : make_uint4(0, 0, 0, 0);
+        qf[t][2 * k][half] = v.x;
+        qf[t][2 * k][2 + half] = v.y;
+        qf[t][2 * k + 1][half] = v.z;
+        qf[t][2 * k + 1][2 + half] = v.w;
+      }
+    }
+
+  float acc[MT][16][4], m[MT][2], l[MT][2];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+  }
+  bool ok = true;
+  int s = 0, turn = 0;
+  for (int i = 0; i < mine; ++i) {
+    ok = __all_sync(kFull, mbar_wait(&full[warp][s], turn, &failed));
+    if (!ok) break;
+    const unsigned char *kb = ring + s * kStageBytes, *vb = kb + 2 * kBoxBytes;
+    const int tile = worker + i * kWorkers, key0 = first_key(tile), end = tile < front_tiles ? front : kv_len;
+    float sc[MT][2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[t][u][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 v = piece(kb + k / 2 * kBoxBytes, 8 * u + n, 2 * c + k % 2);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          product<IS_BF16>(sc[t][u], qf[t][2 * k], v.x, v.y);
+          product<IS_BF16>(sc[t][u], qf[t][2 * k + 1], v.z, v.w);
+        }
+      }
+    }
+    // what a row does not see: keys behind its own position, or between the first tokens and its window; or no key of the walk
+    const bool edge = key0 + kTile > end || p.Sq > 1 || off < 0;
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 8 * u + 2 * c + (e & 1), p_row = at[t][e >> 1];
+            if (key >= end || key > p_row || (key <= p_row - p.window && key >= p.sinks)) sc[t][u][e] = -INFINITY;
+          }
+    }
+    uint32_t pr[MT][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float top[2], f[2];
+      bool grow = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = fmaxf(fmaxf(sc[t][0][2 * h], sc[t][0][2 * h + 1]), fmaxf(sc[t][1][2 * h], sc[t][1][2 * h + 1]));
+        x = fmaxf(x, __shfl_xor_sync(kFull, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(kFull, x, 2)) * p.scale_log2;  // scale > 0: scaling commutes with the maximum
+        // the reference moves only when it would grow by more than 2^8 (the last division makes a stale one exact)
+        top[h] = x > m[t][h] + 8.f ? x : m[t][h];
+        f[h] = top[h] == m[t][h] ? 1.f : fast_exp2(m[t][h] - top[h]);  // (0 at first)
+        grow = grow || top[h] != m[t][h];
+      }
+      if (__any_sync(kFull, grow)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[t][h] *= f[h];
+          m[t][h] = top[h];
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[t][j][e] *= f[e >> 1];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float ref = m[t][h] == -INFINITY ? 0.f : m[t][h];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float a = fast_exp2(fmaf(sc[t][u][2 * h], p.scale_log2, -ref)), z = fast_exp2(fmaf(sc[t][u][2 * h + 1], p.scale_log2, -ref));
+          l[t][h] += a + z;
+          pr[t][2 * u + h] = tc::round_pair<IS_BF16>(a, z);
+        }
+      }
+    }
+    // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dimensions 8n .. 8n + 7 of each half; product j takes dimension 8n + j
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint4 v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = 2 * c + (e & 1) + (e >> 1) * 8;
+        v[e] = piece(vb + half * kBoxBytes, key, n);
+        if (edge && key0 + key >= end) v[e] = make_uint4(0, 0, 0, 0);  // (a probability of 0 times whatever lies there)
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned pick = j & 1 ? 0x7632u : 0x5410u;
+        const uint32_t b0 = __byte_perm(word(v[0], j / 2), word(v[1], j / 2), pick), b1 = __byte_perm(word(v[2], j / 2), word(v[3], j / 2), pick);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) product<IS_BF16>(acc[t][half * 8 + j], pr[t], b0, b1);
+      }
+    }
+    __syncwarp();  // (the whole warp has read the tile)
+    if (lane == 0 && i + kStages < mine) ask(i + kStages);
+    if (++s == kStages) {
+      s = 0;
+      turn ^= 1;
+    }
+  }
+  if (!ok) {  // what this warp has under way ends before its block leaves
+    failed = 1;
+    for (int i = 0; i < kStages; ++i) {
+      const int last = mine - 1 - i;
+      if (last >= 0) mbar_wait(&full[warp][last % kStages], (last / kStages) & 1);
+    }
+  }
+
+  // ---- the warps' sums: the ring makes room for them
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[t][h] += __shfl_xor_sync(kFull, l[t][h], 1);
+      l[t][h] += __shfl_xor_sync(kFull, l[t][h], 2);
+    }
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(smem);  // [kWarps][kRows][kPitch], then the block's [kRows][kPitch]
+  static_assert((kWarps + 1) * kRows * kPitch * sizeof(float) <= (size_t)kWarps * kStages * kStageBytes, "the partial sums take the ring's place");
+  float* block_sums = sums + kWarps * kRows * kPitch;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = t * 16 + h * 8 + n;
+      if (c == 0) {
+        m_part[warp][r] = m[t][h];
+        l_part[warp][r] = l[t][h];
+      }
+      float* dst = sums + (warp * kRows + r) * kPitch;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int j = 0; j < 8; j += 4)  // column 2c + e of product j: dimension 8 (2c + e) + j
+            *reinterpret_cast<float4*>(dst + half * 64 + (2 * c + e) * 8 + j) =
+                make_float4(acc[t][half * 8 + j][2 * h + e], acc[t][half * 8 + j + 1][2 * h + e], acc[t][half * 8 + j + 2][2 * h + e],
+                            acc[t][half * 8 + j + 3][2 * h + e]);
+    }
+  __syncthreads();
+  const int rows = min(kRows, p.rows - row0);
+  auto finish = [&](int r, float4 x, float top, float total) {
+    const int g = (row0 + r) / p.Sq, i = row0 + r - g * p.Sq, h = hk * p.share + g;
+    const float inv = total == 0.f ? 0.f : 1.f / total;  // (a sum may be NaN)
+    uint2 out;
+    out.x = tc::round_pair<IS_BF16>(x.x * inv, x.y * inv);
+    out.y = tc::round_pair<IS_BF16>(x.z * inv, x.w * inv);
+    *reinterpret_cast<uint2*>(p.o + 2 * (b * p.o_sb + h * p.o_sh + i * p.o_ss) + lane * 8) = out;
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[((long long)b * p.H + h) * p.Sq + i] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994530942f;
+  };
+  // a warp a row, a lane four columns
+  for (int r = warp; r < rows; r += kWarps) {
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_part[w][r]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = m_part[w][r] == -INFINITY ? 0.f : fast_exp2(m_part[w][r] - top);
+      const float4 y = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * kPitch + lane * 4);
+      total = fmaf(f, l_part[w][r], total);
+      x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+    }
+    if constexpr (CLUSTER == 1) {
+      finish(r, x, top, total);
+    } else {
+      *reinterpret_cast<float4*>(block_sums + r * kPitch + lane * 4) = x;
+      if (lane == 0) {
+        m_block[r] = top;
+        l_block[r] = total;
+      }
+    }
+  }
+  if constexpr (CLUSTER > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    for (int r = rank + warp * CLUSTER; r < rows; r += CLUSTER * kWarps) {
+      float top = -INFINITY, total = 0.f, ms[CLUSTER], ls[CLUSTER];
+      float4 y[CLUSTER];
+#pragma unroll
+      for (int k = 0; k < CLUSTER; ++k) {
+        ms[k] = ld_cluster_f32(map_to_rank(&m_block[r], k));
+        ls[k] = ld_cluster_f32(map_to_rank(&l_block[r], k));
+        y[k] = ld_cluster_f32x4(map_to_rank(block_sums + r * kPitch + lane * 4, k));
+        top = fmaxf(top, ms[k]);
+      }
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < CLUSTER; ++k) {
+        const float f = ms[k] == -INFINITY ? 0.f : fast_exp2(ms[k] - top);
+        total = fmaf(f, ls[k], total);
+        x.x = fmaf(f, y[k].x, x.x), x.y = fmaf(f, y[k].y, x.y), x.z = fmaf(f, y[k].z, x.z), x.w = fmaf(f, y[k].w, x.w);
+      }
+      finish(r, x, top, total);
+    }
+    __syncwarp();
+    cluster_sync_all();  // nobody leaves while another block reads its shared memory
+  }
+  if (threadIdx.x == 0 && failed && p.status != nullptr) atomicExch(p.status, 1);
+}
+
+template <bool IS_BF16, int MT, int CLUSTER>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, long long items, cudaStream_t stream) {
+  auto kern = window_decode_kernel<IS_BF16, MT, CLUSTER>;
+  static std::atomic<bool> configured[64];
+  int devid = 0;
+  cudaGetDevice(&devid);
+  if (!configured[devid & 63].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    if (e != cudaSuccess) return ixb_host::cuda_status(e);
+    configured[devid & 63].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  cfg.gridDim = dim3((unsigned)(items * CLUSTER));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CLUSTER;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CLUSTER > 1 ? 1 : 0;
+  return ixb_host::cuda_status(cudaLaunchKernelEx(&cfg, kern, mk, mv, p));
+}
+
+}  // namespace
+
+namespace ixb_host {
+
+bool window_decodes(const WindowShape& a) { return (long long)a.Sq * (a.H / a.HK) <= 64; }
+
+int window_decode(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
+                  float* lse, int32_t* status, cudaStream_t stream) {
+  const ixb_devinfo* dev = current_device();
+  if (dev == nullptr) return IXB_ERR_CUDA;
+  CUtensorMap mk, mv;
+  if (int st = make_fa_map(&mk, k.ptr, a.is_bf16, a.B, a.HK, a.Sk, k.strides[0], k.strides[1], k.strides[2], kTile)) return st;
+  if (int st = make_fa_map(&mv, v.ptr, a.is_bf16, a.B, a.HK, a.Sk, v.strides[0], v.strides[1], v.strides[2], kTile)) return st;
+  DecodeParams p;
+  p.q = static_cast<const unsigned char*>(q.ptr);
+  p.o = static_cast<unsigned char*>(const_cast<void*>(o.ptr));
+  p.lse = lse;
+  p.status = status;
+  p.q_lengths = a.q_lengths;
+  p.kv_lengths = a.kv_lengths;
+  p.q_sb = q.strides[0], p.q_sh = q.strides[1], p.q_ss = q.strides[2];
+  p.o_sb = o.strides[0], p.o_sh = o.strides[1], p.o_ss = o.strides[2];
+  p.H = a.H, p.HK = a.HK, p.share = a.H / a.HK, p.Sq = a.Sq, p.Sk = a.Sk;
+  p.rows = p.share * a.Sq;
+  p.scale_log2 = a.scale * kLog2e;
+  p.window = a.window, p.sinks = a.sinks;
+  const int mt = p.rows <= 16 ? 1 : 2;
+  p.groups = (p.rows + 16 * mt - 1) / (16 * mt);
+  const long long items = (long long)a.B * a.HK * p.groups;
+  if (items > (1 << 27)) return IXB_ERR_SHAPE;
+  const long long keys = (long long)a.window + a.Sq - 1 + a.sinks < a.Sk ? a.window + a.Sq - 1 + a.sinks : a.Sk;
+  const long long tiles = (keys + kTile - 1) / kTile;
+  int cluster = 1;
+  while (cluster < 8 && items * cluster < 2 * dev->sm_count && tiles > kWarps * cluster) cluster *= 2;
+  static const int forced = [] { const char* e = getenv("IXB_DECODE_CLUSTER"); return e != nullptr ? atoi(e) : 0; }();
+  if (forced) cluster = forced;
+#define IXB_DECODE_CASE(M, C)    \
+  if (mt == M && cluster == C)   \
+    return a.is_bf16 ? launch<true, M, C>(mk, mv, p, items, stream) : launch<false, M, C>(mk, mv, p, items, stream);
+  IXB_DECODE_CASE(1, 1)
+  IXB_DECODE_CASE(1, 2)
+  IXB_DECODE_CASE(1, 4)
+  IXB_DECODE_CASE(1, 8)
+  IXB_DECODE_CASE(2, 1)
+  IXB_DECODE_CASE(2, 2)
+  IXB_DECODE_CASE(2, 4)
+  IXB_DECODE_CASE(2, 8)
+#undef IXB_DECODE_CASE
+  return IXB_ERR_UNSUPPORTED;
+}
+
+}  // namespace ixb_host

@@ -494,5 +494,7 @@ extern "C" int ixb_window_attention(int dtype, const void* q, const void* k, con
   const ixb_host::WindowView views[] = {{q, q_strides}, {k, k_strides}, {v, v_strides}, {o, o_strides}};
   if (int st = ixb_host::check_window_views(views, 4)) return st;
   const ixb_host::WindowShape a{dtype == IXB_BF16, B, H, HK, Sq, Sk, q_lengths, kv_lengths, scale, window < Sk ? window : Sk, sinks};
+  if (ixb_host::window_decodes(a))
+    return ixb_host::window_decode(a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
   return ixb_host::window_prefill(a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
 }
