@@ -1,15 +1,16 @@
 // Windowed attention of a few queries over a long cache: the decoding step (the meaning of the arguments: fa_window.h).
-// All that a key head's queries need is read once: the rows of a block are those of every query head that shares the key
-// head (R = queries x sharing heads, in groups of 16 x MT), and the keys are the first tokens that lie in front of the
-// window and the window itself, cut into tiles of 16.  The tiles are shared over the kWarps warps of 1, 2, 4 or 8 blocks of a
-// cluster.  A warp keeps its own running maximum, sum and accumulators and has its own ring of copies: nothing waits
-// for another warp before the end, when the warps of a block and then the blocks of the cluster add up, row by row
-// through distributed shared memory: one launch, no scratch, the same bits every time.
+// All that a key head's queries need is read once: a block takes the queries of every query head that shares the key head
+// (queries x sharing heads, in groups of 8 or 16), and the keys are the first tokens that lie in front of the window and the
+// window itself, cut into tiles of 16.  The tiles are shared over the kWarps warps of 1, 2, 4 or 8 blocks of a cluster.  A warp
+// keeps its own running maximum, sum and accumulators and has its own ring of copies: nothing waits for another warp
+// before the end, when the warps of a block and then the blocks of the cluster add up, row by row through distributed
+// shared memory: one launch, no scratch, the same bits every time.
 //
 // Bound: memory.  A key costs 512 bytes and, per row, 512 multiplications, so that warp-wide 16 x 8 x 16 products are
-// enough.  Both operands of both products come out of shared memory as whole 16-byte pieces: the order of the reduced
-// dimensions of S = Q K^T is free, so a lane's piece of 8 dimensions is taken for four of its pairs; the columns of
-// O = P V are free too, so a lane pairs up its pieces of two keys element by element.
+// enough.  They are taken with the keys (S^T = K Q^T) and the dimensions (O^T = V^T P^T) as their 16 rows and the queries as
+// their 8 columns, since hardly more than 8 queries share a key.  K and V come out of shared memory as whole 16-byte
+// pieces: the order of the reduced dimensions of S is free, so a lane's piece of 8 dimensions is taken for four of its pairs;
+// the rows of O are free too, so a lane pairs up its pieces of two keys element by element.
 #include <atomic>
 #include "fa_window.h"
 #include "ixb/tcgen05.cuh"
@@ -31,7 +32,7 @@ struct DecodeParams {
   int* status;    // may be null
   const int *q_lengths, *kv_lengths;
   long long q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;  // elements
-  int H, HK, share, Sq, Sk, rows, groups;        // rows = share * Sq, in `groups` of 16 * MT
+  int H, HK, share, Sq, Sk, rows, groups;        // rows = share * Sq, in `groups` of 8 * NT
   float scale_log2;
   int window, sinks;
 };
@@ -70,16 +71,22 @@ template <bool IS_BF16> __device__ __forceinline__ void product(float (&d)[4], c
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the 8 x 8 matrix of which a lane holds two neighbours of row lane / 4, the other way round
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // piece `chunk` (16 bytes of 8 dimensions) of key `key` in a box of 128-byte rows that the copy engine has swizzled
 __device__ __forceinline__ uint4 piece(const unsigned char* box, int key, int chunk) {
   return *reinterpret_cast<const uint4*>(box + key * 128 + ((chunk ^ (key & 7)) << 4));
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-template <bool IS_BF16, int MT, int CLUSTER>
+template <bool IS_BF16, int NT, int CLUSTER>
 __global__ void __launch_bounds__(kThreads, 2)
     window_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeParams p) {
-  constexpr int kRows = 16 * MT;
+  constexpr int kRows = 8 * NT;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -110,9 +117,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   __syncthreads();
   unsigned char* ring = smem + warp * kStages * kStageBytes;
-  auto ask = [&](int i) {  // tile i of this warp (one lane)
-    unsigned char* dst = ring + i % kStages * kStageBytes;
-    uint64_t* bar = &full[warp][i % kStages];
+  auto ask = [&](int i, int place) {  // tile i of this warp (one lane)
+    unsigned char* dst = ring + place * kStageBytes;
+    uint64_t* bar = &full[warp][place];
     const int key = first_key(worker + i * kWorkers);
     mbar_arrive_expect_tx(bar, kStageBytes);
     tc::tma_load_4d(dst, &map_k, bar, 0, key, hk, b);
@@ -121,34 +128,38 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc::tma_load_4d(dst + 3 * kBoxBytes, &map_v, bar, 64, key, hk, b);
   };
   if (lane == 0)
-    for (int i = 0; i < kStages && i < mine; ++i) ask(i);
+    for (int i = 0; i < kStages && i < mine; ++i) ask(i, i);
 
-  // Q: rows n and n + 8 of each 16.  Piece 2c + odd of a half of 64 dimensions is two of the lane's steps of 16.
-  uint32_t qf[MT][8][4];
-  int at[MT][2];  // position of the row's query (below 0: sees nothing)
+  // Q: the column n of each 8.  Piece 2c + odd of a half of 64 dimensions is two of the lane's steps of 16.
+  uint32_t qf[NT][8][2];
+  int at[NT][2];  // positions of the queries 2c and 2c + 1 (below 0: sees nothing)
+  auto position = [&](int r) {
+    const int i = r % p.Sq;
+    return r < p.rows && i < q_len ? off + i : -1;
+  };
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int t = 0; t < NT; ++t) {
+    const int r = row0 + t * 8 + n, g = r / p.Sq, i = r - g * p.Sq;
+    const bool live = r < p.rows && i < q_len;
+    const unsigned char* src = p.q + 2 * (b * p.q_sb + (hk * p.share + g) * p.q_sh + i * p.q_ss);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = row0 + t * 16 + half * 8 + n, g = r / p.Sq, i = r - g * p.Sq;
-      const bool live = r < p.rows && i < q_len;
-      at[t][half] = live ? off + i : -1;
-      const unsigned char* src = p.q + 2 * (b * p.q_sb + (hk * p.share + g) * p.q_sh + i * p.q_ss);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint4 v = live ? ldg_keep(src + 2 * (k / 2 * 64 + (2 * c + k % 2) * 8)) : make_uint4(0, 0, 0, 0);
-        qf[t][2 * k][half] = v.x;
-        qf[t][2 * k][2 + half] = v.y;
-        qf[t][2 * k + 1][half] = v.z;
-        qf[t][2 * k + 1][2 + half] = v.w;
-      }
+    for (int k = 0; k < 4; ++k) {
+      const uint4 v = live ? ldg_keep(src + 2 * (k / 2 * 64 + (2 * c + k % 2) * 8)) : make_uint4(0, 0, 0, 0);
+      qf[t][2 * k][0] = v.x;
+      qf[t][2 * k][1] = v.y;
+      qf[t][2 * k + 1][0] = v.z;
+      qf[t][2 * k + 1][1] = v.w;
     }
+    at[t][0] = position(row0 + t * 8 + 2 * c);
+    at[t][1] = position(row0 + t * 8 + 2 * c + 1);
+  }
 
-  float acc[MT][16][4], m[MT][2], l[MT][2];
+  // acc: product j, dimensions 8n + j and 64 + 8n + j of the queries 2c and 2c + 1
+  float acc[NT][8][4], m[NT][2], l[NT][2];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
+  for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
     m[t][0] = m[t][1] = -INFINITY;
@@ -161,48 +172,48 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!ok) break;
     const unsigned char *kb = ring + s * kStageBytes, *vb = kb + 2 * kBoxBytes;
     const int tile = worker + i * kWorkers, key0 = first_key(tile), end = tile < front_tiles ? front : kv_len;
-    float sc[MT][2][4];
+    float sc[NT][4];  // keys n (0, 1) and n + 8 (2, 3) of the queries 2c and 2c + 1
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int e = 0; e < 4; ++e) sc[t][e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[t][u][e] = 0.f;
+    for (int k = 0; k < 4; ++k) {
+      const uint4 x = piece(kb + k / 2 * kBoxBytes, n, 2 * c + k % 2), y = piece(kb + k / 2 * kBoxBytes, 8 + n, 2 * c + k % 2);
+      const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint4 v = piece(kb + k / 2 * kBoxBytes, 8 * u + n, 2 * c + k % 2);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          product<IS_BF16>(sc[t][u], qf[t][2 * k], v.x, v.y);
-          product<IS_BF16>(sc[t][u], qf[t][2 * k + 1], v.z, v.w);
-        }
+      for (int t = 0; t < NT; ++t) {
+        product<IS_BF16>(sc[t], a0, qf[t][2 * k][0], qf[t][2 * k][1]);
+        product<IS_BF16>(sc[t], a1, qf[t][2 * k + 1][0], qf[t][2 * k + 1][1]);
       }
     }
-    // what a row does not see: keys behind its own position, or between the first tokens and its window; or no key of the walk
-    const bool edge = key0 + kTile > end || p.Sq > 1 || off < 0;
+    // what a query does not see: keys behind its own position, or between the first tokens and its window; or no key of the walk
+    const bool edge = key0 + kTile > end || p.Sq > 1;
     if (edge) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = key0 + 8 * u + 2 * c + (e & 1), p_row = at[t][e >> 1];
-            if (key >= end || key > p_row || (key <= p_row - p.window && key >= p.sinks)) sc[t][u][e] = -INFINITY;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + n + (e >> 1) * 8, place = at[t][e & 1];
+          if (key >= end || key > place || (key <= place - p.window && key >= p.sinks)) sc[t][e] = -INFINITY;
+        }
     }
-    uint32_t pr[MT][4];
+    uint32_t pr[NT][2];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      float top[2], f[2];
+    for (int t = 0; t < NT; ++t) {
+      float top[2], f[2], x[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[h] = fmaxf(sc[t][h], sc[t][2 + h]);
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[h] = fmaxf(x[h], __shfl_xor_sync(kFull, x[h], o));
       bool grow = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float x = fmaxf(fmaxf(sc[t][0][2 * h], sc[t][0][2 * h + 1]), fmaxf(sc[t][1][2 * h], sc[t][1][2 * h + 1]));
-        x = fmaxf(x, __shfl_xor_sync(kFull, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(kFull, x, 2)) * p.scale_log2;  // scale > 0: scaling commutes with the maximum
+        x[h] *= p.scale_log2;  // scale > 0: scaling commutes with the maximum
         // the reference moves only when it would grow by more than 2^8 (the last division makes a stale one exact)
-        top[h] = x > m[t][h] + 8.f ? x : m[t][h];
+        top[h] = x[h] > m[t][h] + 8.f ? x[h] : m[t][h];
         f[h] = top[h] == m[t][h] ? 1.f : fast_exp2(m[t][h] - top[h]);  // (0 at first)
         grow = grow || top[h] != m[t][h];
       }
@@ -213,41 +224,42 @@ __global__ void __launch_bounds__(kThreads, 2)
           m[t][h] = top[h];
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[t][j][e] *= f[e >> 1];
+          for (int e = 0; e < 4; ++e) acc[t][j][e] *= f[e & 1];
       }
+      const float ref[2] = {m[t][0] == -INFINITY ? 0.f : m[t][0], m[t][1] == -INFINITY ? 0.f : m[t][1]};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float ref = m[t][h] == -INFINITY ? 0.f : m[t][h];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float a = fast_exp2(fmaf(sc[t][u][2 * h], p.scale_log2, -ref)), z = fast_exp2(fmaf(sc[t][u][2 * h + 1], p.scale_log2, -ref));
-          l[t][h] += a + z;
-          pr[t][2 * u + h] = tc::round_pair<IS_BF16>(a, z);
-        }
+      for (int u = 0; u < 2; ++u) {
+        const float a = fast_exp2(fmaf(sc[t][2 * u], p.scale_log2, -ref[0])), z = fast_exp2(fmaf(sc[t][2 * u + 1], p.scale_log2, -ref[1]));
+        l[t][0] += a;
+        l[t][1] += z;
+        pr[t][u] = transposed(tc::round_pair<IS_BF16>(a, z));  // keys 2c, 2c + 1 (and 8 behind them) of query n
       }
     }
-    // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dimensions 8n .. 8n + 7 of each half; product j takes dimension 8n + j
+    // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dimensions 8n .. 8n + 7 of each half; product j takes dimension 8n + j of both
+    uint4 v[2][4];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint4 v[4];
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = 2 * c + (e & 1) + (e >> 1) * 8;
-        v[e] = piece(vb + half * kBoxBytes, key, n);
-        if (edge && key0 + key >= end) v[e] = make_uint4(0, 0, 0, 0);  // (a probability of 0 times whatever lies there)
+        v[half][e] = piece(vb + half * kBoxBytes, key, n);
+        if (edge && key0 + key >= end) v[half][e] = make_uint4(0, 0, 0, 0);  // (a probability of 0 times whatever lies there)
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const unsigned pick = j & 1 ? 0x7632u : 0x5410u;
-        const uint32_t b0 = __byte_perm(word(v[0], j / 2), word(v[1], j / 2), pick), b1 = __byte_perm(word(v[2], j / 2), word(v[3], j / 2), pick);
+    for (int j = 0; j < 8; ++j) {
+      const unsigned pick = j & 1 ? 0x7632u : 0x5410u;
+      uint32_t a[4];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) product<IS_BF16>(acc[t][half * 8 + j], pr[t], b0, b1);
-      }
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) a[2 * u + half] = __byte_perm(word(v[half][2 * u], j / 2), word(v[half][2 * u + 1], j / 2), pick);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) product<IS_BF16>(acc[t][j], a, pr[t][0], pr[t][1]);
     }
     __syncwarp();  // (the whole warp has read the tile)
-    if (lane == 0 && i + kStages < mine) ask(i + kStages);
+    if (lane == 0 && i + kStages < mine) ask(i + kStages, s);
     if (++s == kStages) {
       s = 0;
       turn ^= 1;
@@ -255,30 +267,29 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (!ok) {  // what this warp has under way ends before its block leaves
     failed = 1;
-    for (int i = 0; i < kStages; ++i) {
-      const int last = mine - 1 - i;
-      if (last >= 0) mbar_wait(&full[warp][last % kStages], (last / kStages) & 1);
+    for (int i = 1; i < kStages; ++i) {
+      const int other = (s + i) % kStages;
+      mbar_wait(&full[warp][other], s + i < kStages ? turn : turn ^ 1);
     }
   }
 
   // ---- the warps' sums: the ring makes room for them
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[t][h] += __shfl_xor_sync(kFull, l[t][h], 1);
-      l[t][h] += __shfl_xor_sync(kFull, l[t][h], 2);
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) l[t][h] += __shfl_xor_sync(kFull, l[t][h], o);
   __syncthreads();
   float* sums = reinterpret_cast<float*>(smem);  // [kWarps][kRows][kPitch], then the block's [kRows][kPitch]
   static_assert((kWarps + 1) * kRows * kPitch * sizeof(float) <= (size_t)kWarps * kStages * kStageBytes, "the partial sums take the ring's place");
   float* block_sums = sums + kWarps * kRows * kPitch;
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = t * 16 + h * 8 + n;
-      if (c == 0) {
+      const int r = t * 8 + 2 * c + h;
+      if (n == 0) {
         m_part[warp][r] = m[t][h];
         l_part[warp][r] = l[t][h];
       }
@@ -286,12 +297,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int j = 0; j < 8; j += 4)  // column 2c + e of product j: dimension 8 (2c + e) + j
-            *reinterpret_cast<float4*>(dst + half * 64 + (2 * c + e) * 8 + j) =
-                make_float4(acc[t][half * 8 + j][2 * h + e], acc[t][half * 8 + j + 1][2 * h + e], acc[t][half * 8 + j + 2][2 * h + e],
-                            acc[t][half * 8 + j + 3][2 * h + e]);
+        for (int j = 0; j < 8; j += 4)
+          *reinterpret_cast<float4*>(dst + half * 64 + 8 * n + j) =
+              make_float4(acc[t][j][2 * half + h], acc[t][j + 1][2 * half + h], acc[t][j + 2][2 * half + h], acc[t][j + 3][2 * half + h]);
     }
   __syncthreads();
   const int rows = min(kRows, p.rows - row0);
@@ -356,9 +364,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (threadIdx.x == 0 && failed && p.status != nullptr) atomicExch(p.status, 1);
 }
 
-template <bool IS_BF16, int MT, int CLUSTER>
+template <bool IS_BF16, int NT, int CLUSTER>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, long long items, cudaStream_t stream) {
-  auto kern = window_decode_kernel<IS_BF16, MT, CLUSTER>;
+  auto kern = window_decode_kernel<IS_BF16, NT, CLUSTER>;
   static std::atomic<bool> configured[64];
   int devid = 0;
   cudaGetDevice(&devid);
@@ -386,7 +394,39 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, 
 
 namespace ixb_host {
 
-bool window_decodes(const WindowShape& a) { return (long long)a.Sq * (a.H / a.HK) <= 64; }
+// Keys that the queries of a sequence see at most.
+static long long keys_seen(const WindowShape& a) {
+  const long long keys = (long long)a.window + a.Sq - 1 + a.sinks;
+  return keys < a.Sk ? keys : a.Sk;
+}
+static int clusters_of(long long items, long long tiles, int sms) {
+  int cluster = 1;
+  while (cluster < 8 && items * cluster <= sms && tiles > kWarps * cluster) cluster *= 2;
+  return cluster;
+}
+
+// Whether this kernel promises to be quicker than fa_window_fwd.cu, as measured on one B200 (35 shapes of 16 to 128 rows a key
+// head, 8 to 512 key heads, within 15 %), in us:
+//   that one   8 + 1.7 a step of 128 keys for each round of its items over the SMs
+//   this one   5 + 0.6 a tile of a warp, and not less than 1.25 for each 8 tiles an SM
+// 16 rows, 8 key heads, 1024 keys 24.2 against 6.8, 4096 keys 63 and 12.3; 64 rows, 64 key heads, 1024 keys 24.6 and 23.2, 256 key heads,
+// 2048 keys 71 and 142; 128 rows, 8 key heads, 4096 keys 62 and 23, 64 key heads, 1024 keys 24.9 and 44.5.
+bool window_decodes(const WindowShape& a) {
+  const long long share = a.H / a.HK, rows = share * a.Sq;
+  if (rows > 256) return false;
+  const ixb_devinfo* dev = current_device();
+  if (dev == nullptr) return true;
+  const double sms = dev->sm_count, heads = (double)a.B * a.HK, keys = (double)keys_seen(a);
+  const int groups = rows <= 8 ? 1 : (int)((rows + 15) / 16);
+  const long long tiles = ((long long)keys + 2 * kTile - 2) / kTile;
+  const int cluster = clusters_of((long long)heads * groups, tiles, dev->sm_count);
+  const double chain = 0.6 * tiles / (kWarps * cluster), load = 1.25 * heads * groups * tiles / (8 * sms);
+  int rows_of_head = 8;
+  while (rows_of_head < 128 && rows_of_head < a.Sq) rows_of_head *= 2;
+  const double pairs = ceil((double)((a.Sq + 127) / 128) * ceil((double)share * rows_of_head / 128) / 2);
+  const double steps = ceil(keys / 128) + (a.sinks > 0 ? 2 : 1);
+  return 5 + (chain > load ? chain : load) < 8 + 1.7 * steps * ceil(heads * pairs / sms);
+}
 
 int window_decode(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
                   float* lse, int32_t* status, cudaStream_t stream) {
@@ -408,19 +448,13 @@ int window_decode(const WindowShape& a, const WindowView& q, const WindowView& k
   p.rows = p.share * a.Sq;
   p.scale_log2 = a.scale * kLog2e;
   p.window = a.window, p.sinks = a.sinks;
-  const int mt = p.rows <= 16 ? 1 : 2;
-  p.groups = (p.rows + 16 * mt - 1) / (16 * mt);
+  const int nt = p.rows <= 8 ? 1 : 2;
+  p.groups = (p.rows + 8 * nt - 1) / (8 * nt);
   const long long items = (long long)a.B * a.HK * p.groups;
   if (items > (1 << 27)) return IXB_ERR_SHAPE;
-  const long long keys = (long long)a.window + a.Sq - 1 + a.sinks < a.Sk ? a.window + a.Sq - 1 + a.sinks : a.Sk;
-  const long long tiles = (keys + kTile - 1) / kTile;
-  int cluster = 1;
-  while (cluster < 8 && items * cluster < 2 * dev->sm_count && tiles > kWarps * cluster) cluster *= 2;
-  static const int forced = [] { const char* e = getenv("IXB_DECODE_CLUSTER"); return e != nullptr ? atoi(e) : 0; }();
-  if (forced) cluster = forced;
-#define IXB_DECODE_CASE(M, C)    \
-  if (mt == M && cluster == C)   \
-    return a.is_bf16 ? launch<true, M, C>(mk, mv, p, items, stream) : launch<false, M, C>(mk, mv, p, items, stream);
+  const int cluster = clusters_of(items, (keys_seen(a) + 2 * kTile - 2) / kTile, dev->sm_count);
+#define IXB_DECODE_CASE(N, C) \
+  if (nt == N && cluster == C) return a.is_bf16 ? launch<true, N, C>(mk, mv, p, items, stream) : launch<false, N, C>(mk, mv, p, items, stream);
   IXB_DECODE_CASE(1, 1)
   IXB_DECODE_CASE(1, 2)
   IXB_DECODE_CASE(1, 4)

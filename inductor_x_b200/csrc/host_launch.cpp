@@ -153,15 +153,23 @@ decltype(&ixb_rmsnorm) entry_rmsnorm;
 decltype(&ixb_fa_fwd) entry_fa_fwd;
 decltype(&ixb_fa_bwd_scratch_bytes) entry_fa_bwd_room;
 decltype(&ixb_fa_bwd_scratch) entry_fa_bwd;
+decltype(&ixb_rmsnorm_quantised) entry_rmsnorm_quantised;
+decltype(&ixb_axial_rotary) entry_rotary;
+decltype(&ixb_window_attention) entry_window;
+decltype(&ixb_window_attention_scratch_bytes) entry_window_room;
+decltype(&ixb_window_attention_bwd) entry_window_bwd;
+decltype(&ixb_window_attention_bwd_scratch_bytes) entry_window_bwd_room;
 
-// bind_library(rmsnorm, fa_fwd, fa_bwd_scratch_bytes, fa_bwd_scratch): addresses of the C entries
+// bind_library(rmsnorm, fa_fwd, fa_bwd_scratch_bytes, fa_bwd_scratch, rmsnorm_quantised, axial_rotary, window_attention and its
+// scratch_bytes, window_attention_bwd and its scratch_bytes): addresses of the C entries
 PyObject* bind_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  void* p[4];
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "bind_library takes four addresses");
+  constexpr int kEntries = 10;
+  void* p[kEntries];
+  if (n != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "bind_library takes ten addresses");
     return nullptr;
   }
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kEntries; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr && PyErr_Occurred()) return nullptr;
   }
@@ -169,6 +177,12 @@ PyObject* bind_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   entry_fa_fwd = reinterpret_cast<decltype(entry_fa_fwd)>(p[1]);
   entry_fa_bwd_room = reinterpret_cast<decltype(entry_fa_bwd_room)>(p[2]);
   entry_fa_bwd = reinterpret_cast<decltype(entry_fa_bwd)>(p[3]);
+  entry_rmsnorm_quantised = reinterpret_cast<decltype(entry_rmsnorm_quantised)>(p[4]);
+  entry_rotary = reinterpret_cast<decltype(entry_rotary)>(p[5]);
+  entry_window = reinterpret_cast<decltype(entry_window)>(p[6]);
+  entry_window_room = reinterpret_cast<decltype(entry_window_room)>(p[7]);
+  entry_window_bwd = reinterpret_cast<decltype(entry_window_bwd)>(p[8]);
+  entry_window_bwd_room = reinterpret_cast<decltype(entry_window_bwd_room)>(p[9]);
   Py_RETURN_NONE;
 }
 
@@ -332,9 +346,206 @@ PyObject* fused_attention_backward(PyObject*, PyObject* const* args, Py_ssize_t 
   }
 }
 
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) {
+    PyObject* x = out ? THPVariable_Wrap(t) : nullptr;
+    if (x == nullptr) {
+      Py_XDECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i++, x);
+  }
+  return out;
+}
+// a small whole number, or -1
+int64_t count_of(PyObject* o) {
+  if (!PyLong_CheckExact(o)) return -1;
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) PyErr_Clear();
+  return v < 0 ? -1 : v;
+}
+
+// rms_norm_quantised(x, w, eps, residual or None, return_residual, group)
+PyObject* rms_norm_quantised(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || entry_rmsnorm_quantised == nullptr || observed() || !PyFloat_CheckExact(args[2]) || !PyBool_Check(args[4])) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x = plain_tensor(args[0]), *w = plain_tensor(args[1]);
+    const int64_t group = count_of(args[5]);
+    if (x == nullptr || w == nullptr || x->dim() < 1 || !x->is_contiguous() || dtype_code(*x) < 0 || (group != 0 && group != 128)) Py_RETURN_NONE;
+    const int64_t cols = x->size(-1), rows = cols ? x->numel() / cols : 0;
+    if (rows == 0 || !alike(*x, *w) || w->dim() != 1 || w->size(0) != cols || !w->is_contiguous()) Py_RETURN_NONE;
+    const at::Tensor* r = nullptr;
+    if (args[3] != Py_None) {
+      r = plain_tensor(args[3]);
+      if (r == nullptr || !alike(*x, *r) || r->sizes() != x->sizes() || !r->is_contiguous()) Py_RETURN_NONE;
+    }
+    std::vector<int64_t> lead(x->sizes().begin(), x->sizes().end() - 1);
+    if (group) lead.push_back((cols + group - 1) / group);
+    at::Tensor q = at::empty(x->sizes(), x->options().dtype(at::kFloat8_e4m3fn)), scales = at::empty(lead, x->options().dtype(at::kFloat)), h;
+    if (r != nullptr && args[4] == Py_True) h = at::empty_like(*x);
+    const ixb_stream stream = stream_of(*x);
+    const float eps = (float)PyFloat_AS_DOUBLE(args[2]);
+    const c10::OptionalDeviceGuard device(x->device());
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = entry_rmsnorm_quantised(dtype_code(*x), x->data_ptr(), r ? r->data_ptr() : nullptr, w->data_ptr(), q.data_ptr(),
+                                 static_cast<float*>(scales.data_ptr()), h.defined() ? h.data_ptr() : nullptr, rows, cols, (int32_t)group, eps, stream);
+    Py_END_ALLOW_THREADS
+    if (st != 0) return PyLong_FromLong(st);
+    return h.defined() ? tuple_of({q, scales, h}) : tuple_of({q, scales});
+  } catch (...) {
+    return left_to_python();
+  }
+}
+
+// axial_rotary(q, k or None, positions, pairs, axes, address of the sections, address of the frequencies, neighbours, inverse)
+PyObject* axial_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9 || entry_rotary == nullptr || observed() || !PyBool_Check(args[7]) || !PyBool_Check(args[8])) Py_RETURN_NONE;
+  try {
+    const at::Tensor *q = plain_tensor(args[0]), *k = args[1] == Py_None ? nullptr : plain_tensor(args[1]), *pos = plain_tensor(args[2]);
+    const int64_t pairs = count_of(args[3]), axes = count_of(args[4]);
+    void *sections = PyLong_AsVoidPtr(args[5]), *frequencies = PyLong_AsVoidPtr(args[6]);
+    if (PyErr_Occurred()) return left_to_python();
+    if (q == nullptr || pos == nullptr || (k == nullptr && args[1] != Py_None) || pairs < 1 || axes < 1 || sections == nullptr || frequencies == nullptr)
+      Py_RETURN_NONE;
+    auto dense = [&](const at::Tensor& t) {  // (an expanded input is left to Python)
+      return t.dim() == 4 && t.stride(3) == 1 && t.numel() > 0 && t.stride(0) > 0 && t.stride(1) > 0 && t.stride(2) > 0;
+    };
+    if (dtype_code(*q) < 0 || !dense(*q) || 2 * pairs > q->size(3) || q->device() != pos->device()) Py_RETURN_NONE;
+    if (k != nullptr && (!dense(*k) || !alike(*q, *k) || k->size(0) != q->size(0) || k->size(2) != q->size(2) || k->size(3) != q->size(3)))
+      Py_RETURN_NONE;
+    const int64_t B = q->size(0), S = q->size(2);
+    if (B * S > INT32_MAX || q->size(1) > INT32_MAX || (k != nullptr && k->size(1) > INT32_MAX)) Py_RETURN_NONE;
+    const bool all = pos->dim() == 2;
+    if ((!all && pos->dim() != 3) || pos->size(0) != axes || (!all && pos->size(1) != B) || pos->size(-1) != S ||
+        (pos->scalar_type() != at::kLong && pos->scalar_type() != at::kInt))
+      Py_RETURN_NONE;
+    const int64_t at_strides[3] = {pos->stride(0), all ? 0 : pos->stride(1), pos->stride(-1)};
+    at::Tensor qo = at::empty_like(*q), ko;
+    if (k != nullptr) ko = at::empty_like(*k);
+    const Strides qs(*q), qos(qo), ks(k ? *k : *q), kos(k ? ko : qo);
+    const ixb_stream stream = stream_of(*q);
+    const c10::OptionalDeviceGuard device(q->device());
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = entry_rotary(dtype_code(*q), q->data_ptr(), qo.data_ptr(), qs.v, qos.v, (int32_t)q->size(1), k ? k->data_ptr() : nullptr,
+                      k ? ko.data_ptr() : nullptr, ks.v, kos.v, k ? (int32_t)k->size(1) : 0, pos->data_ptr(),
+                      pos->scalar_type() == at::kLong ? IXB_I64 : IXB_I32, at_strides, (int32_t)B, (int32_t)S, (int32_t)q->size(3), (int32_t)axes,
+                      static_cast<const int32_t*>(sections), static_cast<const double*>(frequencies), args[7] == Py_True, args[8] == Py_True, stream);
+    Py_END_ALLOW_THREADS
+    if (st != 0) return PyLong_FromLong(st);
+    return k ? pair(std::move(qo), std::move(ko)) : THPVariable_Wrap(std::move(qo));
+  } catch (...) {
+    return left_to_python();
+  }
+}
+
+// What both directions of the windowed attention take: q[B, H, Sq, D], k and v [B, HK, Sk, D], lengths int32[B] or None.
+struct WindowCall {
+  const at::Tensor *q, *k, *v, *q_lengths = nullptr, *kv_lengths = nullptr;
+  int32_t B, H, HK, Sq, Sk, window, sinks;
+  bool ok = false;
+  WindowCall(PyObject* const* t, PyObject* window_arg, PyObject* sinks_arg, PyObject* ql, PyObject* kl)
+      : q(plain_tensor(t[0])), k(plain_tensor(t[1])), v(plain_tensor(t[2])) {
+    if (!q || !k || !v || q->dim() != 4 || k->dim() != 4 || k->sizes() != v->sizes() || q->size(0) != k->size(0) || q->size(3) != 128 ||
+        k->size(3) != 128 || k->size(1) == 0 || q->size(1) % k->size(1) != 0 || dtype_code(*q) <= IXB_F32 || !alike(*q, *k) || !alike(*q, *v) ||
+        q->numel() == 0 || k->numel() == 0 || q->stride(3) != 1 || k->stride(3) != 1 || v->stride(3) != 1 || q->numel() > INT32_MAX * (int64_t)128 ||
+        k->numel() > INT32_MAX * (int64_t)128)
+      return;
+    const int64_t w = count_of(window_arg), s = count_of(sinks_arg);
+    if (w < 1 || s < 0 || s > 128) return;
+    if (!lengths(ql, q_lengths) || !lengths(kl, kv_lengths)) return;
+    B = (int32_t)q->size(0), H = (int32_t)q->size(1), HK = (int32_t)k->size(1), Sq = (int32_t)q->size(2), Sk = (int32_t)k->size(2);
+    window = (int32_t)(w < INT32_MAX ? w : INT32_MAX);
+    sinks = (int32_t)s;
+    ok = true;
+  }
+  bool lengths(PyObject* o, const at::Tensor*& t) const {
+    if (o == Py_None) return true;
+    t = plain_tensor(o);
+    return t != nullptr && t->dim() == 1 && t->size(0) == q->size(0) && t->scalar_type() == at::kInt && t->device() == q->device() && t->is_contiguous();
+  }
+  static const int32_t* ptr(const at::Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
+};
+// Strides; an axis of one entry, whose stride says nothing, counts as dense.
+struct OperandStrides {
+  int64_t v[3];
+  explicit OperandStrides(const at::Tensor& t)
+      : v{t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2) * t.size(3), t.size(1) > 1 ? t.stride(1) : t.size(2) * t.size(3),
+          t.size(2) > 1 ? t.stride(2) : t.size(3)} {}
+};
+
+// window_attention(q, k, v, scale, window, sinks, q_lengths or None, kv_lengths or None, return_lse)
+PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9 || entry_window == nullptr || observed() || !PyFloat_CheckExact(args[3]) || !PyBool_Check(args[8])) Py_RETURN_NONE;
+  try {
+    const WindowCall c(args, args[4], args[5], args[6], args[7]);
+    if (!c.ok) Py_RETURN_NONE;
+    at::Tensor out = at::empty({c.B, c.H, c.Sq, 128}, c.q->options()), lse;
+    if (args[8] == Py_True) lse = at::empty({c.B, c.H, c.Sq}, c.q->options().dtype(at::kFloat));
+    const size_t room = entry_window_room(c.B, c.H, c.HK, c.Sq, c.Sk, c.window, c.sinks);
+    const c10::OptionalDeviceGuard device(c.q->device());
+    c10::DataPtr scratch;  // memory as it is (see fused_attention_backward)
+    if (room) scratch = c10::GetAllocator(c10::kCUDA)->allocate(room);
+    const OperandStrides qs(*c.q), ks(*c.k), vs(*c.v), os(out);
+    const ixb_stream stream = stream_of(*c.q);
+    const float scale = (float)PyFloat_AS_DOUBLE(args[3]);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = entry_window(dtype_code(*c.q), c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), out.data_ptr(),
+                      lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, scratch.get(), room, c.B, c.H, c.HK, c.Sq, c.Sk, 128, qs.v, ks.v,
+                      vs.v, os.v, WindowCall::ptr(c.q_lengths), WindowCall::ptr(c.kv_lengths), scale, c.window, c.sinks, nullptr, stream);
+    Py_END_ALLOW_THREADS
+    if (st != 0) return PyLong_FromLong(st);
+    return lse.defined() ? pair(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
+  } catch (...) {
+    return left_to_python();
+  }
+}
+
+// window_attention_backward(q, k, v, out, lse, dout, scale, window, sinks, q_lengths or None, kv_lengths or None)
+PyObject* window_attention_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 11 || entry_window_bwd == nullptr || observed() || !PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
+  try {
+    const WindowCall c(args, args[7], args[8], args[9], args[10]);
+    const at::Tensor *o = plain_tensor(args[3]), *lse = plain_tensor(args[4]), *go = plain_tensor(args[5]);
+    if (!c.ok || !o || !lse || !go || o->sizes() != c.q->sizes() || go->sizes() != c.q->sizes() || !alike(*c.q, *o) || !alike(*c.q, *go) ||
+        o->stride(3) != 1 || go->stride(3) != 1)
+      Py_RETURN_NONE;
+    const OperandStrides qs(*c.q), ks(*c.k), vs(*c.v), os(*o), gs(*go);
+    for (int i = 0; i < 3; ++i)
+      if (gs.v[i] <= 0 || gs.v[i] % 8 != 0) Py_RETURN_NONE;
+    if (lse->dim() != 3 || lse->size(0) != c.B || lse->size(1) != c.H || lse->size(2) != c.Sq || lse->scalar_type() != at::kFloat ||
+        lse->device() != c.q->device() || !lse->is_contiguous())
+      Py_RETURN_NONE;
+    at::Tensor dq = at::empty({c.B, c.H, c.Sq, 128}, c.q->options()), dk = at::empty({c.B, c.HK, c.Sk, 128}, c.q->options()),
+               dv = at::empty({c.B, c.HK, c.Sk, 128}, c.q->options());
+    const size_t room = entry_window_bwd_room(c.B, c.H, c.HK, c.Sq, c.Sk, c.window, c.sinks);
+    const c10::OptionalDeviceGuard device(c.q->device());
+    const c10::DataPtr scratch = c10::GetAllocator(c10::kCUDA)->allocate(room);
+    const OperandStrides dqs(dq), dks(dk), dvs(dv);
+    const ixb_stream stream = stream_of(*c.q);
+    const float scale = (float)PyFloat_AS_DOUBLE(args[6]);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = entry_window_bwd(dtype_code(*c.q), c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), o->data_ptr(), go->data_ptr(),
+                          static_cast<const float*>(lse->data_ptr()), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), scratch.get(), room, c.B, c.H,
+                          c.HK, c.Sq, c.Sk, 128, qs.v, ks.v, vs.v, os.v, gs.v, dqs.v, dks.v, dvs.v, WindowCall::ptr(c.q_lengths),
+                          WindowCall::ptr(c.kv_lengths), scale, c.window, c.sinks, nullptr, stream);
+    Py_END_ALLOW_THREADS
+    if (st != 0) return PyLong_FromLong(st);
+    return tuple_of({dq, dk, dv});
+  } catch (...) {
+    return left_to_python();
+  }
+}
+
 #define IXB_FASTCALL(fn) {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef functions[] = {IXB_FASTCALL(bind_library), IXB_FASTCALL(rms_norm), IXB_FASTCALL(fused_attention),
-                           IXB_FASTCALL(fused_attention_backward), {nullptr, nullptr, 0, nullptr}};
+                           IXB_FASTCALL(fused_attention_backward), IXB_FASTCALL(rms_norm_quantised), IXB_FASTCALL(axial_rotary),
+                           IXB_FASTCALL(window_attention), IXB_FASTCALL(window_attention_backward), {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
 

@@ -350,6 +350,9 @@ def rmsnorm_quantised(x, w, eps: float = 1e-6, *, residual=None, return_residual
     (``torch.float8_e4m3fn``, the shape of ``x``) times ``scales`` (float32) the norm of ``h``.  ``group=0``: a scale
     for each row, ``scales`` of shape ``x.shape[:-1]``; ``group=128``: one for each 128 values, ``[..., ceil(cols /
     128)]``.  A scale is the largest magnitude / 448; the norm is rounded once, to 8 bits."""
+    done = _native("ixb_rmsnorm_quantised", _ixb_host.rms_norm_quantised(x, w, eps, residual, return_residual, group))
+    if done is not None:
+        return done
     _need_cuda(x, w, residual)
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError(f"unsupported dtype {x.dtype}")
@@ -432,6 +435,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     are read.
 
     Returns ``out`` (contiguous ``[B, H, Sq, D]``) or ``(out, lse)``; ``check=True`` as in :func:`fused_attention`."""
+    if not check:
+        done = _native("ixb_window_attention", _ixb_host.window_attention(q, k, v, scale, window, sinks, q_lengths, kv_lengths, return_lse))
+        if done is not None:
+            return done
     window, sinks, q_lengths, kv_lengths = _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths)
     B, H, Sq, D = q.shape
     HK, Sk = k.shape[1], k.shape[2]
@@ -461,6 +468,11 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """Gradients ``(dq, dk, dv)`` of :func:`window_attention` from its inputs, its output ``out``, its log-sum-exp
     ``lse`` (``return_lse=True``) and the incoming gradient ``dout``; ``dk`` and ``dv`` are sums over the query heads
     that share a key head, and zero where no query sees the key.  Deterministic, no atomics."""
+    if not check:
+        done = _native("ixb_window_attention_bwd", _ixb_host.window_attention_backward(
+            q, k, v, out, lse, dout, scale, window, sinks, q_lengths, kv_lengths))
+        if done is not None:
+            return done
     window, sinks, q_lengths, kv_lengths = _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths)
     _need_cuda(out, lse, dout)
     if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype:
@@ -500,7 +512,7 @@ PAIRINGS, LADDERS = ("halves", "neighbours"), ("shared", "own")
 
 @functools.lru_cache(maxsize=256)
 def _rotary_plan(sections: tuple, base: float, ladder: str, frequencies: Optional[tuple]):
-    """(pairs, axes, ctypes sections, ctypes frequencies in radians a position)."""
+    """(pairs, axes, ctypes sections, ctypes frequencies in radians a position, their addresses)."""
     pairs = sum(sections)
     if not sections or any(n < 0 for n in sections) or not 1 <= pairs <= 128:
         raise ValueError("sections must be one count of pairs for each axis, 1 to 128 together")
@@ -511,15 +523,19 @@ def _rotary_plan(sections: tuple, base: float, ladder: str, frequencies: Optiona
         frequencies = tuple(base ** -p for p in powers)
     if len(frequencies) != pairs:
         raise ValueError("frequencies must be one number for each pair")
-    return pairs, len(sections), (ctypes.c_int32 * len(sections))(*sections), (ctypes.c_double * pairs)(*frequencies)
+    c_sections, c_frequencies = (ctypes.c_int32 * len(sections))(*sections), (ctypes.c_double * pairs)(*frequencies)
+    return (pairs, len(sections), c_sections, c_frequencies, ctypes.addressof(c_sections), ctypes.addressof(c_frequencies))
 
 
 def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inverse):
-    _need_cuda(q, k, positions)
     if pairing not in PAIRINGS or ladder not in LADDERS:
         raise ValueError(f"pairing must be one of {PAIRINGS}, ladder one of {LADDERS}")
-    pairs, axes, c_sections, c_frequencies = _rotary_plan(
+    pairs, axes, c_sections, c_frequencies, *addresses = _rotary_plan(
         tuple(sections), float(base), ladder, tuple(frequencies) if frequencies is not None else None)
+    done = _native("ixb_axial_rotary", _ixb_host.axial_rotary(q, k, positions, pairs, axes, *addresses, pairing == "neighbours", inverse))
+    if done is not None:
+        return done
+    _need_cuda(q, k, positions)
     if q.dtype not in (torch.float32, torch.float16, torch.bfloat16) or (k is not None and k.dtype != q.dtype):
         raise ValueError("q and k must share dtype float32, float16 or bfloat16")
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):

@@ -148,7 +148,9 @@ def load() -> ctypes.CDLL:
     from . import _ixb_host
 
     _ixb_host.bind_library(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
-        "ixb_rmsnorm", "ixb_fa_fwd", "ixb_fa_bwd_scratch_bytes", "ixb_fa_bwd_scratch")))
+        "ixb_rmsnorm", "ixb_fa_fwd", "ixb_fa_bwd_scratch_bytes", "ixb_fa_bwd_scratch", "ixb_rmsnorm_quantised", "ixb_axial_rotary",
+        "ixb_window_attention", "ixb_window_attention_scratch_bytes", "ixb_window_attention_bwd",
+        "ixb_window_attention_bwd_scratch_bytes")))
     _lib = lib
     return lib
 
