@@ -6,8 +6,10 @@
 // power of two that holds all of the call's queries where they are fewer (8 at least).  The tiles of a key
 // head, those of the same rows one after the other, go two to an item, so that with an even number of
 // sharing heads both tiles of an item see the very same keys and every tile of K and V serves both.
-// An item walks the first key tile, where it is not in the window but has first tokens, and the key tiles from the
-// one its window begins in to the one its last row stands in.  A tile of rows leaves out those that only the other one sees.
+// An item walks the key tiles back from the one its last row stands in to the one its window begins in: every row sees its
+// own position, so that the running maximum is near its end from the first step on and accumulators are hardly ever
+// rescaled.  The first key tile, where that is not in the window but has first tokens, is the second step; up to kFront
+// first tokens take copies, products and exponentials of kFront keys only.  A tile of rows leaves out steps that only the other one sees.
 //
 // What lies behind a sequence's length in K and V may be anything: scores of hidden keys are replaced before they are
 // looked at, but a probability of 0 times a NaN is one, so the producer clears the rows of V behind the length in the
@@ -21,9 +23,11 @@ namespace {
 using namespace ixb;
 using namespace ixb::fa;
 
+constexpr int kFront = 32;  // keys of a short last step
+constexpr int kFrontBytes = kFront * HD * 2;
 constexpr int kStages = 2;  // (the issuer picks stage descriptors with two-way selects)
 // Registers: as in fa_fwd.cu
-constexpr int kRegsLaunch = 168, kRegsIssue = 80, kRegsSoftmax = 208;
+constexpr int kRegsLaunch = 168, kRegsIssue = 88, kRegsSoftmax = 208;
 static_assert(kRegsIssue + NQ * kRegsSoftmax <= (1 + NQ) * kRegsLaunch, "setmaxnreg draws on the block's own registers");
 constexpr size_t kSmemBytes = (size_t)kTileBytes * (NQ + 2 * kStages) + 1024;
 
@@ -39,6 +43,7 @@ struct WinParams {
   int rows_log2;         // R = 1 << rows_log2 rows of a head in a tile
   int tiles;             // tiles of rows a key head has
   int wide;
+  int head_group;        // key heads whose items are dispatched together
 };
 
 // Of a row at position `at`: keys of the tile behind `lim` are hidden, and those in [from, low), the ones between the first
@@ -46,12 +51,12 @@ struct WinParams {
 struct WindowMask {
   bool edge;
   int lim, from, low;
-  __device__ __forceinline__ void apply(uint32_t (&raw)[BN]) const {
+  template <int COLS> __device__ __forceinline__ void apply(uint32_t (&raw)[COLS]) const {
     if (!edge) return;
     // the first n keys of 32
     auto first = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
 #pragma unroll
-    for (int c = 0; c < BN / 32; ++c) {
+    for (int c = 0; c < COLS / 32; ++c) {
       const uint32_t seen = first(lim + 1 - c * 32) & ~(first(low - c * 32) & ~first(from - c * 32));
       if (__all_sync(kFull, seen == 0xffffffffu)) continue;
 #pragma unroll
@@ -64,7 +69,8 @@ struct WindowMask {
 template <bool IS_BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     fa_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                         const __grid_constant__ CUtensorMap map_v, const WinParams p) {
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kf,
+                         const __grid_constant__ CUtensorMap map_vf, const WinParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -86,19 +92,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     int b, hk, off, q_len, kv_len;   // query i stands at position off + i
     int i0[NQ], h0[NQ];              // first row and first head of each tile (h0 < 0: no such tile)
     int lo[NQ], hi[NQ];              // key tiles of each tile's window (none: hi = 0)
-    int lo_all, n_kv, first;         // first: the walk begins with key tile 0, which is in no window
+    int lo_all, end, n_kv, front;    // key tiles [lo_all, end), and with `front` tile 0, which is in no window
   };
   auto item_of = [&](int index) {
     Item w;
     const int per_head = (p.tiles + NQ - 1) / NQ;
-    const int bh = index / per_head, n = per_head - 1 - (index - bh * per_head);  // late (long) ones of a head first
+    const int group = index / (per_head * p.head_group), in_group = index - group * per_head * p.head_group;
+    const int g_heads = min(p.head_group, p.B * p.HK - group * p.head_group);
+    const int bh = group * p.head_group + in_group % g_heads, n = per_head - 1 - in_group / g_heads;
     w.b = bh / p.HK;
     w.hk = bh - w.b * p.HK;
     w.q_len = p.q_lengths != nullptr ? min(max(__ldg(p.q_lengths + w.b), 0), p.Sq) : p.Sq;
     w.kv_len = p.kv_lengths != nullptr ? min(max(__ldg(p.kv_lengths + w.b), 0), p.Sk) : p.Sk;
     w.off = w.kv_len - w.q_len;
     w.lo_all = 1 << 30;
-    int end = 0;
+    w.end = 0;
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       const int u = NQ * n + t, i = u / blocks_of_heads;
@@ -111,21 +119,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       w.hi[t] = any ? last / BN + 1 : 0;
       if (any) {
         w.lo_all = min(w.lo_all, w.lo[t]);
-        end = max(end, w.hi[t]);
+        w.end = max(w.end, w.hi[t]);
       }
     }
-    w.first = end > 0 && w.lo_all > 0 && p.sinks > 0 ? 1 : 0;
-    w.n_kv = end > 0 ? end - w.lo_all + w.first : 0;
+    w.front = w.end > 0 && w.lo_all > 0 && p.sinks > 0 ? 1 : 0;
+    w.n_kv = w.end > 0 ? w.end - w.lo_all + w.front : 0;
     return w;
   };
-  // key tile of step x of an item, and whether tile t of rows looks at it
-  auto key_tile = [&](const Item& w, int x) { return w.first ? (x == 0 ? 0 : w.lo_all + x - 1) : w.lo_all + x; };
-  auto looks = [&](const Item& w, int t, int x) {
-    if (x >= w.n_kv) return false;
-    const int j = key_tile(w, x);
-    const int lo = t ? w.lo[1] : w.lo[0], hi = t ? w.hi[1] : w.hi[0];
-    return hi > 0 && j < hi && (j >= lo || (j == 0 && p.sinks > 0));
-  };
+  // key tile of step x of an item: the first tokens' is the second
+  auto key_tile = [&](const Item& w, int x) { return !w.front ? w.end - 1 - x : x == 0 ? w.end - 1 : x == 1 ? 0 : w.end - x; };
 
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
@@ -200,13 +202,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int x = 0; x < w.n_kv; ++x, ++step) {
           const int s = step & 1, u = step >> 1, j = key_tile(w, x);
+          const bool brief = w.front && p.sinks <= kFront && x == 1;
           ok = u == 0 || __all_sync(kFull, mbar_wait(&k_empty[s], (u - 1) & 1, &failed));
           if (!ok) break;
           if (lane == 0) {
+            // (a short step's keys are the first kFront rows of each box)
             unsigned char* kd = k_smem + (size_t)s * kTileBytes;
-            mbar_arrive_expect_tx(&k_full[s], kTileBytes);
-            tc::tma_load_4d(kd, &map_k, &k_full[s], 0, j * BN, w.hk, w.b);
-            tc::tma_load_4d(kd + kHalfBytes, &map_k, &k_full[s], 64, j * BN, w.hk, w.b);
+            const CUtensorMap* map = brief ? &map_kf : &map_k;
+            mbar_arrive_expect_tx(&k_full[s], brief ? kFrontBytes : kTileBytes);
+            tc::tma_load_4d(kd, map, &k_full[s], 0, j * BN, w.hk, w.b);
+            tc::tma_load_4d(kd + kHalfBytes, map, &k_full[s], 64, j * BN, w.hk, w.b);
             if (x + 1 == w.n_kv) tc::mbar_arrive(&next_wanted);
           }
           k_loads = step + 1;
@@ -214,12 +219,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           unsigned char* vd = v_smem + (size_t)s * kTileBytes;
           const int live = w.kv_len - j * BN;
-          const bool clear = live < BN && w.kv_len < p.Sk;  // the tile reaches behind the sequence, and not behind the tensor
+          // the tile reaches behind the sequence, and not behind the tensor (the first one does not, where it is in no window)
+          const bool clear = live < BN && w.kv_len < p.Sk;
           uint64_t* bar = clear ? &v_raw : &v_full[s];
           if (lane == 0) {
-            mbar_arrive_expect_tx(bar, kTileBytes);
-            tc::tma_load_4d(vd, &map_v, bar, 0, j * BN, w.hk, w.b);
-            tc::tma_load_4d(vd + kHalfBytes, &map_v, bar, 64, j * BN, w.hk, w.b);
+            const CUtensorMap* map = brief ? &map_vf : &map_v;
+            mbar_arrive_expect_tx(bar, brief ? kFrontBytes : kTileBytes);
+            tc::tma_load_4d(vd, map, bar, 0, j * BN, w.hk, w.b);
+            tc::tma_load_4d(vd + kHalfBytes, map, bar, 64, j * BN, w.hk, w.b);
           }
           if (clear) {
             raw_pending = true;
@@ -247,15 +254,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       // -------------------------------------------------------------------- MMA issuer
       // The whole warp runs this role and an elected lane issues (see tc::product_ss).
       constexpr uint32_t idesc_qk = tc::instr_desc(BM, BN, IS_BF16 ? 1 : 0, 0, 0);
+      constexpr uint32_t idesc_front = tc::instr_desc(BM, kFront, IS_BF16 ? 1 : 0, 0, 0);
       constexpr uint32_t idesc_pv = tc::instr_desc(BM, HD, IS_BF16 ? 1 : 0, 0, 1);
       const uint32_t tmem = __shfl_sync(kFull, tmem_base, 0);
       const uint64_t q_desc = tc::smem_desc(smem_u32(q_smem), 16, 1024);
       const uint64_t k_desc = tc::smem_desc(smem_u32(k_smem), 16, 1024);
       const uint64_t v_desc = tc::smem_desc(smem_u32(v_smem), kHalfBytes, 1024);
       // tile t, stage s: the address field moves by whole tiles and cannot carry out of it
-      auto issue_qk = [&](int t, int stage) {
+      auto issue_qk = [&](int t, int stage, bool brief) {
         tc::product_ss<kHalfBytes>(tmem + kColS + t * 128, q_desc + (uint32_t)(t * (kTileBytes >> 4)),
-                                   k_desc + (uint32_t)(stage * (kTileBytes >> 4)), idesc_qk);
+                                   k_desc + (uint32_t)(stage * (kTileBytes >> 4)), brief ? idesc_front : idesc_qk);
         tc::commit_elected(&s_full[t]);
       };
       bool ok = true;
@@ -263,8 +271,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       int items = 0;              // items with keys so far
       int products[NQ] = {0, 0};  // P tiles consumed so far
       for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
-        const Item w = item_of(index);
-        if (w.n_kv > 0) {
+        int n_kv, first[NQ], behind[NQ], last[NQ];  // window steps [first, behind) of a tile of rows, and its last one
+        bool front, brief;                          // step 1 is the first tokens', and short
+        {
+          const Item w = item_of(index);
+          n_kv = w.n_kv;
+          front = w.front != 0;
+          brief = front && p.sinks <= kFront;
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            auto step_of = [&](int j) { return front && j < w.end - 1 ? w.end - j : w.end - 1 - j; };
+            const bool any = w.hi[t] > 0;
+            first[t] = any ? step_of(w.hi[t] - 1) : n_kv;
+            behind[t] = any ? step_of(w.lo[t]) + 1 : n_kv;
+            last[t] = !any ? -1 : front ? max(1, behind[t] - 1) : w.lo[t] > 0 && p.sinks > 0 ? n_kv - 1 : behind[t] - 1;
+          }
+        }
+        auto looks = [&](int t, int x) { return (x >= first[t] && x < behind[t]) || x == last[t] || (front && x == 1 && last[t] > 0); };
+        bool begun[NQ] = {false, false};
+        if (n_kv > 0) {
           ok = __all_sync(kFull, mbar_wait(&q_full, items & 1, &failed)) &&
                __all_sync(kFull, mbar_wait(&k_full[step & 1], (step >> 1) & 1, &failed));
           if (!ok) break;
@@ -272,48 +297,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::fence_after_sync();
 #pragma unroll
           for (int t = 0; t < NQ; ++t)
-            if (looks(w, t, 0)) issue_qk(t, step & 1);
+            if (looks(t, 0)) issue_qk(t, step & 1, false);  // (the last row's own tile: never the short step)
           tc::commit_elected(&k_empty[step & 1]);
-          if (w.n_kv == 1) tc::commit_elected(&q_empty);
+          if (n_kv == 1) tc::commit_elected(&q_empty);
         }
-        bool begun[NQ] = {false, false};
-        for (int x = 0; x < w.n_kv; ++x) {
+        for (int x = 0; x < n_kv; ++x) {
           const int s = (step + x) & 1, u = (step + x) >> 1;
           const int s1 = (step + x + 1) & 1, u1 = (step + x + 1) >> 1;
           ok = __all_sync(kFull, mbar_wait(&v_full[s], u & 1, &failed));
-          if (x + 1 < w.n_kv) ok = ok && __all_sync(kFull, mbar_wait(&k_full[s1], u1 & 1, &failed));
+          if (x + 1 < n_kv) ok = ok && __all_sync(kFull, mbar_wait(&k_full[s1], u1 & 1, &failed));
           if (!ok) break;
+          const bool brief_now = brief && x == 1, brief_next = brief && x == 0;
 #pragma unroll
           for (int t = 0; t < NQ; ++t) {
-            const bool do_qk = looks(w, t, x + 1);
-            if (looks(w, t, x)) {
+            if (looks(t, x)) {
               // O_t += P_t V_j in two parts, as in fa_fwd.cu
               ok = ok && __all_sync(kFull, mbar_wait(&p_full[t], products[t] & 1, &failed));
               if (!ok) break;
               tc::fence_after_sync();
               const uint64_t vd = v_desc + (uint32_t)(s * (kTileBytes >> 4));
               const uint32_t o = tmem + kColO + t * 128, pa = tmem + kColS + t * 128;
-              tc::product_ts<kSplit / 16>(o, pa, vd, idesc_pv, begun[t]);
+              if (brief_now) tc::product_ts<kFront / 16>(o, pa, vd, idesc_pv, begun[t]);
+              else tc::product_ts<kSplit / 16>(o, pa, vd, idesc_pv, begun[t]);
               ok = __all_sync(kFull, mbar_wait(&p_rest[t], products[t] & 1, &failed));
               if (!ok) break;
               tc::fence_after_sync();
               // (16 keys of V are 2048 bytes of a 64-column box)
-              tc::product_ts<(BN - kSplit) / 16>(o, pa + kSplit / 2, vd + (uint32_t)(kSplit / 16 * 2048 >> 4), idesc_pv, 1u);
+              if (!brief_now) tc::product_ts<(BN - kSplit) / 16>(o, pa + kSplit / 2, vd + (uint32_t)(kSplit / 16 * 2048 >> 4), idesc_pv, 1u);
               ++products[t];
               begun[t] = true;
-              // the tile's last product: the key tile that its last row stands in
-              if (key_tile(w, x) + 1 == (t ? w.hi[1] : w.hi[0])) tc::commit_elected(&pv_done[t]);
+              if (x == last[t]) tc::commit_elected(&pv_done[t]);
             }
             // P_t has been consumed by the MMAs just issued (the tensor core runs them in
             // order), so tile t's buffer can take the scores of the next step
-            if (do_qk) issue_qk(t, s1);
+            if (x + 1 < n_kv && looks(t, x + 1)) issue_qk(t, s1, brief_next);
           }
           if (!ok) break;
           tc::commit_elected(&v_empty[s]);
-          if (x + 1 < w.n_kv) tc::commit_elected(&k_empty[s1]);
-          if (x + 2 == w.n_kv) tc::commit_elected(&q_empty);  // the item's last scores are issued
+          if (x + 1 < n_kv) tc::commit_elected(&k_empty[s1]);
+          if (x + 2 == n_kv) tc::commit_elected(&q_empty);  // the item's last scores are issued
         }
-        step += w.n_kv;
+        step += n_kv;
         index = take_next(n, ok);
       }
       if (!ok && lane == 0) failed = 1;
@@ -346,29 +370,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     int closed = 0; // items in which this tile of rows had work
     for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
       const Item w = item_of(index);
-      const int i0 = t ? w.i0[1] : w.i0[0], h0 = t ? w.h0[1] : w.h0[0], hi = t ? w.hi[1] : w.hi[0];
+      const int i0 = t ? w.i0[1] : w.i0[0], h0 = t ? w.h0[1] : w.h0[0], lo = t ? w.lo[1] : w.lo[0], hi = t ? w.hi[1] : w.hi[0];
       const int qi = i0 + (row & (R - 1)), h = h0 + (row >> p.rows_log2);
       const int at = qi < w.q_len ? w.off + qi : -1;  // (below 0: sees nothing)
       // every row of the tile sees all of a key tile that ends before the first row and begins in the last row's window
       const int at_first = w.off + i0, at_last = w.off + min(i0 + R, w.q_len) - 1;
+      const bool brief = p.sinks <= kFront && w.front;
       float m_used = -INFINITY;  // reference maximum (scaled, log2 domain)
       float l = 0.f;             // running sum of exp2(s - m_used)
-      bool begun = false;
-      for (int x = 0; x < w.n_kv; ++x) {
-        if (!looks(w, t, x)) continue;
+      // key tiles hi - 1 .. lo, and tile 0 where it is not among them but has first tokens: the item's step 1, or its last
+      const int steps = hi - lo + (p.sinks > 0 && lo > 0 ? 1 : 0), front_step = !w.front ? hi - lo : hi == w.end ? 1 : 0;
+      for (int i = 0; i < steps; ++i) {
+        const bool front = i == front_step;
+        const int j = hi - 1 - i + (i > front_step ? 1 : 0);
         if (!__all_sync(kFull, mbar_wait(&s_full[t], seen & 1, &failed))) {
           ok = false;
           break;
         }
         tc::fence_after_sync();
-        const int col0 = key_tile(w, x) * BN;
+        const int col0 = front ? 0 : j * BN;
         WindowMask mask;
-        mask.edge = col0 + BN - 1 > at_first || col0 <= at_last - p.window;
+        mask.edge = front || col0 + BN - 1 > at_first || col0 <= at_last - p.window;
         mask.lim = at - col0;
         mask.from = col0 == 0 ? p.sinks : 0;
         mask.low = at - p.window + 1 - col0;
-        softmax_tile<IS_BF16>(s_addr, o_addr, mask, !begun, p.scale_log2, m_used, l, &p_full[t], &p_rest[t]);
-        begun = true;
+        if (front && brief)
+          softmax_tile<IS_BF16, kFront>(s_addr, o_addr, mask, i == 0, p.scale_log2, m_used, l, &p_full[t], &p_rest[t]);
+        else
+          softmax_tile<IS_BF16>(s_addr, o_addr, mask, i == 0, p.scale_log2, m_used, l, &p_full[t], &p_rest[t]);
         ++seen;
       }
       if (ok && hi > 0) {
@@ -378,23 +407,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && h0 >= 0) {
         tc::fence_after_sync();
         if (at < 0) l = 0.f;  // (tiles that all other rows see whole are not masked)
-        const float inv = (l > 0.f) ? 1.f / l : (l == 0.f ? 0.f : l);  // (l may be NaN)
         const bool live = qi < p.Sq && h < (w.hk + 1) * p.share;
         unsigned char* orow = reinterpret_cast<unsigned char*>(p.o) +
                               2 * ((long long)w.b * p.o_stride_b + (long long)h * p.o_stride_h +
                                    (long long)qi * p.o_stride_s);
+        if (hi > 0) {
+          const float inv = 1.f / l;  // (l may be NaN)
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          if (hi > 0) {
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
             tc::tmem_ld32(o_addr + c * 32, o);
             tc::tmem_wait_ld();
+            if (live && l != 0.f) tc::store_row32<IS_BF16>(orow + c * 64, o, inv, p.wide != 0);
           }
-          if (l == 0.f) {  // nothing was seen
+        }
+        if (live && l == 0.f) {  // nothing was seen
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0;
-          }
-          if (live) tc::store_row32<IS_BF16>(orow + c * 64, o, inv, p.wide != 0);
+          for (int c = 0; c < HD / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
         }
         if (live && p.lse != nullptr) {
           const float lse = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994530942f;  // (l may be NaN)
@@ -443,6 +472,11 @@ int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& 
   if (int st = make_fa_map(&mq, q.ptr, a.is_bf16, a.B, a.H, a.Sq, q.strides[0], q.strides[1], q.strides[2], 1 << p.rows_log2)) return st;
   if (int st = make_fa_map(&mk, k.ptr, a.is_bf16, a.B, a.HK, a.Sk, k.strides[0], k.strides[1], k.strides[2])) return st;
   if (int st = make_fa_map(&mv, v.ptr, a.is_bf16, a.B, a.HK, a.Sk, v.strides[0], v.strides[1], v.strides[2])) return st;
+  CUtensorMap mkf = mk, mvf = mv;
+  if (a.sinks > 0 && a.window < a.Sk) {
+    if (int st = make_fa_map(&mkf, k.ptr, a.is_bf16, a.B, a.HK, a.Sk, k.strides[0], k.strides[1], k.strides[2], kFront)) return st;
+    if (int st = make_fa_map(&mvf, v.ptr, a.is_bf16, a.B, a.HK, a.Sk, v.strides[0], v.strides[1], v.strides[2], kFront)) return st;
+  }
   p.o = const_cast<void*>(o.ptr);
   p.lse = lse;
   p.status = status;
@@ -459,6 +493,7 @@ int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& 
   const long long items = (tiles + NQ - 1) / NQ * a.B * a.HK;
   if (items > 0x7fffffffLL) return IXB_ERR_SHAPE;
   p.tiles = (int)tiles;
+  p.head_group = 8;
   p.wide = rows_aligned32(o.ptr, o.strides) ? 1 : 0;
   auto kern = a.is_bf16 ? fa_window_fwd_kernel<true> : fa_window_fwd_kernel<false>;
   // the shared-memory opt-in is a property of (kernel, device): set once per device
@@ -475,7 +510,7 @@ int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& 
     if (at.numRegs != kRegsLaunch) return IXB_ERR_UNSUPPORTED;
     done.store(true, std::memory_order_release);
   }
-  kern<<<(unsigned)items, kThreads, kSmemBytes, stream>>>(mq, mk, mv, p);
+  kern<<<(unsigned)items, kThreads, kSmemBytes, stream>>>(mq, mk, mv, mkf, mvf, p);
   return cuda_status(cudaGetLastError());
 }
 

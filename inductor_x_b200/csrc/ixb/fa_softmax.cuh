@@ -47,21 +47,21 @@ struct CausalMask {
 // Scores of this thread's row (tensor memory at s_addr) to probabilities relative to the running reference
 // maximum m_used, written over them as 16-bit pairs and handed over in two parts (p_full after kSplit keys,
 // p_rest); l grows by their sum.  `mask` hides keys of the tile from this row.  `first`: the row's accumulator at
-// o_addr holds nothing yet.
-template <bool IS_BF16, class Mask>
+// o_addr holds nothing yet.  COLS: keys of the tile, all or the first 32 of them (which are handed over at once).
+template <bool IS_BF16, int COLS = BN, class Mask>
 __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, const Mask& mask, bool first, float scale_log2,
                                              float& m_used, float& l, uint64_t* p_full, uint64_t* p_rest) {
   // the row of scores stays in registers: one trip through tensor memory per tile
-  uint32_t raw[BN];
+  uint32_t raw[COLS];
 #pragma unroll
-  for (int c = 0; c < BN / 32; ++c)
+  for (int c = 0; c < COLS / 32; ++c)
     tc::tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[c * 32]));
   tc::tmem_wait_ld();
   mask.apply(raw);
   // four independent chains: one chain of 64 dependent max3 would cost its latency 64 times
   float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int e = 0; e < BN; e += 2)
+  for (int e = 0; e < COLS; e += 2)
     mx4[(e >> 1) & 3] = max3(mx4[(e >> 1) & 3], __uint_as_float(raw[e]), __uint_as_float(raw[e + 1]));
   float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
   mx *= scale_log2;  // scale > 0: scaling commutes with the maximum
@@ -93,7 +93,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, c
   const float2 nm2 = make_float2(-mref, -mref);
   float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // two chains of packed adds
 #pragma unroll
-  for (int c = 0; c < BN / 32; ++c) {
+  for (int c = 0; c < COLS / 32; ++c) {
     uint32_t pk[16];
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
@@ -103,7 +103,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, c
       pk[e / 2] = pack_pair(pe.x, pe.y, IS_BF16);
     }
     tc::tmem_st16(s_addr + c * 16, pk);
-    if (c * 32 + 32 == kSplit) {
+    if (c * 32 + 32 == (COLS < kSplit ? COLS : kSplit)) {
       tc::tmem_wait_st();
       tc::fence_before_sync();
       tc::mbar_arrive(p_full);
