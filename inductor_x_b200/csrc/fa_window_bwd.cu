@@ -111,30 +111,41 @@ struct Scheduler {
 };
 
 // ------------------------------------------------------------------------------ delta
+// A block 64 rows of a head.
 template <bool IS_BF16>
 __global__ void __launch_bounds__(256)
-    window_delta_kernel(const unsigned char* o, const unsigned char* dout, float* delta, int H, int Sq, long long rows,
-                        long long o_sb, long long o_sh, long long o_ss, long long d_sb, long long d_sh, long long d_ss) {
-  // half a warp per row: 16 lanes x 16 bytes = the 128 16-bit values of a row
+    window_delta_kernel(const unsigned char* o, const unsigned char* dout, float* delta, int H, int Sq, int blocks, long long o_sb,
+                        long long o_sh, long long o_ss, long long d_sb, long long d_sh, long long d_ss) {
+  // half a warp per row: 16 lanes x 16 bytes = the 128 16-bit values of a row; kRows rows of a half in flight
+  constexpr int kRows = 4;
   const int lane = threadIdx.x & 31, sub = lane & 15;
-  const long long row = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2 + (lane >> 4);
-  float s = 0.f;
-  if (row < rows) {
-    const long long bh = row / Sq;
-    const long long i = row - bh * Sq;
-    const long long b = bh / H, h = bh - b * H;
-    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(o + 2 * (b * o_sb + h * o_sh + i * o_ss) + sub * 16));
-    const uint4 g = ldg_stream(reinterpret_cast<const uint4*>(dout + 2 * (b * d_sb + h * d_sh + i * d_ss) + sub * 16));
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+  // (heads next to each other: in a projection's gradient so are their rows, 256 bytes of a row of all heads)
+  const int bt = blockIdx.x / H, h = blockIdx.x - bt * H, b = bt / blocks, bh = b * H + h;
+  const int row0 = (bt - b * blocks) * 64 + (threadIdx.x >> 5) * 2 * kRows + (lane >> 4);
+  o += 2 * (b * o_sb + h * o_sh) + sub * 16;
+  dout += 2 * (b * d_sb + h * d_sh) + sub * 16;
+  uint4 a[kRows], g[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const int i = row0 + 2 * k;
+    a[k] = g[k] = make_uint4(0, 0, 0, 0);
+    if (i >= Sq) continue;
+    a[k] = ldg_stream(reinterpret_cast<const uint4*>(o + 2 * (i * o_ss)));
+    g[k] = ldg_stream(reinterpret_cast<const uint4*>(dout + 2 * (i * d_ss)));
+  }
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const uint32_t aw[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, gw[4] = {g[k].x, g[k].y, g[k].z, g[k].w};
+    float s = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 x = unpack_pair(aw[e], IS_BF16), y = unpack_pair(gw[e], IS_BF16);
       s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
     }
-  }
 #pragma unroll
-  for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(kFull, s, off);
-  if (sub == 0 && row < rows) delta[row] = s;
+    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(kFull, s, off);
+    if (sub == 0 && row0 + 2 * k < Sq) delta[(long long)bh * Sq + row0 + 2 * k] = s;
+  }
 }
 
 // ------------------------------------------------------------------------------ dK, dV
@@ -977,8 +988,8 @@ extern "C" int ixb_window_attention_bwd(int dtype, const void* q, const void* k,
   p.sinks = sinks;
   p.chunks = sink_chunks(H, HK, Sq, Sk, window, sinks);
   const long long q_tiles = ((long long)Sq + BM - 1) / BM, kv_tiles = ((long long)Sk + BN - 1) / BN;
-  const long long rows = (long long)B * H * Sq, dkv_items = (kv_tiles + p.chunks) * B * HK, dq_items = q_tiles * B * H;
-  if (rows > 0x7fffffffLL * 16 || dkv_items > 0x7fffffffLL || dq_items > 0x7fffffffLL) return IXB_ERR_SHAPE;
+  const long long delta_blocks = ((long long)Sq + 63) / 64 * B * H, dkv_items = (kv_tiles + p.chunks) * B * HK, dq_items = q_tiles * B * H;
+  if (delta_blocks > 0x7fffffffLL || dkv_items > 0x7fffffffLL || dq_items > 0x7fffffffLL) return IXB_ERR_SHAPE;
   const int is_bf16 = dtype == IXB_BF16;
   CUtensorMap mq, mk, mv, mdo;
   if (int st = ixb_host::make_fa_map(&mq, q, is_bf16, B, H, Sq, q_strides[0], q_strides[1], q_strides[2])) return st;
@@ -1009,8 +1020,8 @@ extern "C" int ixb_window_attention_bwd(int dtype, const void* q, const void* k,
   if (int st = opt_in(kern_dkv, configured[0][is_bf16][devid & 63], kDkvSmem)) return st;
   if (int st = opt_in(kern_dq, configured[1][is_bf16][devid & 63], kDqSmem)) return st;
   const cudaStream_t cs = (cudaStream_t)stream;
-  kern_delta<<<(unsigned)((rows + 15) / 16), 256, 0, cs>>>(
-      static_cast<const unsigned char*>(o), static_cast<const unsigned char*>(dout), delta, H, Sq, rows,
+  kern_delta<<<(unsigned)delta_blocks, 256, 0, cs>>>(
+      static_cast<const unsigned char*>(o), static_cast<const unsigned char*>(dout), delta, H, Sq, (Sq + 63) / 64,
       o_strides[0], o_strides[1], o_strides[2], do_strides[0], do_strides[1], do_strides[2]);
   kern_dkv<<<(unsigned)dkv_items, kThreads, kDkvSmem, cs>>>(mq, mk, mv, mdo, p);
   if (p.chunks) {

@@ -42,6 +42,7 @@ struct WinParams {
   int window, sinks;
   int rows_log2;         // R = 1 << rows_log2 rows of a head in a tile
   int tiles;             // tiles of rows a key head has
+  int per_item;          // of which an item takes two, or one
   int wide;
   int head_group;        // key heads whose items are dispatched together
 };
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   auto item_of = [&](int index) {
     Item w;
-    const int per_head = (p.tiles + NQ - 1) / NQ;
+    const int per_head = (p.tiles + p.per_item - 1) / p.per_item;
     const int group = index / (per_head * p.head_group), in_group = index - group * per_head * p.head_group;
     const int g_heads = min(p.head_group, p.B * p.HK - group * p.head_group);
     const int bh = group * p.head_group + in_group % g_heads, n = per_head - 1 - in_group / g_heads;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     w.end = 0;
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-      const int u = NQ * n + t, i = u / blocks_of_heads;
+      const int u = t < p.per_item ? p.per_item * n + t : p.tiles, i = u / blocks_of_heads;
       w.i0[t] = i * BM;  // (fewer rows a head than a tile has: all of them are in tile 0)
       w.h0[t] = u < p.tiles ? w.hk * p.share + ((u - i * blocks_of_heads) << (7 - p.rows_log2)) : -1;
       const int last = w.off + min(w.i0[t] + R, w.q_len) - 1;  // position of the tile's last row, and of its first
@@ -490,7 +491,12 @@ int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& 
   p.window = a.window, p.sinks = a.sinks;
   const int heads = BM >> p.rows_log2;  // query heads in a tile
   const long long tiles = (long long)((a.Sq + BM - 1) / BM) * ((p.share + heads - 1) / heads);
-  const long long items = (tiles + NQ - 1) / NQ * a.B * a.HK;
+  // One tile an item where that leaves no SM with two: a step of one takes about two thirds of a step of both.
+  // 3 x 4 key heads, 500 queries of share 3, window 600: PER_ITEM_FIGURES.
+  const ixb_devinfo* dev = current_device();
+  if (dev == nullptr) return IXB_ERR_CUDA;
+  p.per_item = tiles * a.B * a.HK <= dev->sm_count ? 1 : NQ;
+  const long long items = (tiles + p.per_item - 1) / p.per_item * a.B * a.HK;
   if (items > 0x7fffffffLL) return IXB_ERR_SHAPE;
   p.tiles = (int)tiles;
   p.head_group = 8;
