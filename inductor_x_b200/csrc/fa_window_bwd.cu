@@ -12,8 +12,8 @@
 // each leaves the 32-bit sums of the first tokens' rows in scratch, and window_sinks_kernel adds them up in order.
 // One owner for every sum, no atomics: the bits are the same from run to run.
 //
-// What lies behind a sequence's lengths may be anything.  Q and dO meet every key as operands, K every query: the producers
-// clear their rows behind the length.  V's rows only meet their own, whose results are replaced.
+// What lies behind a sequence's lengths may be anything.  The producers clear such rows of what meets all rows of the other
+// side: Q and dO for dK and dV, K and V for dQ.  The others' only meet their own row of results, which is replaced.
 //
 // Every wait is bounded and raises a flag in `status`; the block leaves when its copies and products have ended.
 #include <atomic>
@@ -440,7 +440,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         float2 pr[GC / 2];
 #pragma unroll
         for (int c = 0; c < GC / 32; ++c) {
-          const uint32_t seen = edge ? first_of(hi - c * 32) & ~first_of(lo - c * 32) : 0xffffffffu;
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
@@ -450,15 +449,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int u = 0; u < 2; ++u) {
               const int at = c * 32 + e + 2 * u;
               const float2 a = fma2(make_float2(__uint_as_float(raw[at]), __uint_as_float(raw[at + 1])), sc2, l2[u]);
-              float2 x = make_float2(fast_exp2(a.x), fast_exp2(a.y));
-              if (edge) {
-                if (!(seen >> (e + 2 * u) & 1u)) x.x = 0.f;
-                if (!(seen >> (e + 2 * u + 1) & 1u)) x.y = 0.f;
-              }
-              pr[at / 2] = x;
-              pk[e / 2 + u] = pack_pair(x.x, x.y, IS_BF16);
+              pr[at / 2] = make_float2(fast_exp2(a.x), fast_exp2(a.y));
             }
           }
+          if (edge) {  // (a branch of its own: inside the loop above it costs every tile its selects)
+            const uint32_t seen = first_of(hi - c * 32) & ~first_of(lo - c * 32);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              if (!(seen >> e & 1u)) pr[c * 16 + e / 2].x = 0.f;
+              if (!(seen >> (e + 1) & 1u)) pr[c * 16 + e / 2].y = 0.f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = pack_pair(pr[c * 16 + e].x, pr[c * 16 + e].y, IS_BF16);
           // all of this group's S columns are in registers: P^T goes over their first half
           tc::tmem_st16(s_addr + c * 16, pk);
         }
@@ -730,9 +733,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (uv > 0) ok = __all_sync(kFull, mbar_wait(&v_empty[sv], (uv - 1) & 1, &failed));
         if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&v_full[sv], kTileBytes);
-          load_tile(v_smem + (size_t)sv * kTileBytes, &map_v, &v_full[sv], j * BN, w.hk, w.b);
+        if (!clear) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&v_full[sv], kTileBytes);
+            load_tile(v_smem + (size_t)sv * kTileBytes, &map_v, &v_full[sv], j * BN, w.hk, w.b);
+          }
+        } else {
+          ok = load_cleared(v_smem + (size_t)sv * kTileBytes, &map_v, &raw_full, raw_loads & 1, &v_full[sv], j * BN, w.hk, w.b, live, lane,
+                            &failed, raw_pending);
+          ++raw_loads;
+          if (!ok) break;
         }
         ++v_loads;
       }
@@ -826,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool some = lse != -INFINITY;
       const float dl = some ? p.delta[stat_at] : 0.f;
       const float nl = some ? -lse * kLog2e : -INFINITY;
-      const float2 nl2 = make_float2(nl, nl);
+      const float2 nl2 = make_float2(nl, nl), ndl2 = make_float2(-dl, -dl);
       const int at_first = w.n.off + w.qt0, at_last = at_first + BM - 1;
       for (int x = 0; x < w.n_kv; ++x, ++step) {
         if (!__all_sync(kFull, mbar_wait(&s_full, step & 1, &failed))) {
@@ -843,16 +853,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j0 = key_tile(w, x) * BN, col0 = j0 + GC * g;
         const bool edge = j0 + BN - 1 > at_first || j0 <= at_last - p.window || w.qt0 + BM > w.n.q;
         const int lim = at - col0, low = at - p.window + 1 - col0, from = (j0 == 0 ? p.sinks : 0) - GC * g;
-        uint32_t seen[GC / 32];
-        float pr[GC];
+        float2 pr[GC / 2];
 #pragma unroll
-        for (int c = 0; c < GC / 32; ++c) {
-          seen[c] = edge ? first_of(lim + 1 - c * 32) & ~(first_of(low - c * 32) & ~first_of(from - c * 32)) : 0xffffffffu;
+        for (int e = 0; e < GC; e += 2) {
+          const float2 a = fma2(make_float2(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), sc2, nl2);
+          pr[e / 2] = make_float2(fast_exp2(a.x), fast_exp2(a.y));
+        }
+        if (edge) {
 #pragma unroll
-          for (int e = c * 32; e < c * 32 + 32; e += 2) {
-            const float2 a = fma2(make_float2(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), sc2, nl2);
-            pr[e] = fast_exp2(a.x);
-            pr[e + 1] = fast_exp2(a.y);
+          for (int c = 0; c < GC / 32; ++c) {
+            const uint32_t seen = first_of(lim + 1 - c * 32) & ~(first_of(low - c * 32) & ~first_of(from - c * 32));
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              if (!(seen >> e & 1u)) pr[c * 16 + e / 2].x = 0.f;
+              if (!(seen >> (e + 1) & 1u)) pr[c * 16 + e / 2].y = 0.f;
+            }
           }
         }
         if (!__all_sync(kFull, mbar_wait(&dp_full[step & 1], (step >> 1) & 1, &failed))) {
@@ -869,13 +884,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float x0 = pr[c * 32 + e] * (__uint_as_float(d[e]) - dl);
-            float x1 = pr[c * 32 + e + 1] * (__uint_as_float(d[e + 1]) - dl);
-            if (edge) {  // (hidden keys may hold anything)
-              if (!(seen[c] >> e & 1u)) x0 = 0.f;
-              if (!(seen[c] >> (e + 1) & 1u)) x1 = 0.f;
-            }
-            pk[e / 2] = pack_pair(x0, x1, IS_BF16);
+            const float2 x = mul2(pr[c * 16 + e / 2], add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), ndl2));
+            pk[e / 2] = pack_pair(x.x, x.y, IS_BF16);
           }
           tc::tmem_st16(dp_addr + c * 16, pk);
         }
