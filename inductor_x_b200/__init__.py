@@ -9,7 +9,7 @@ Drop-in for the registration surface of BD-Seed-HHW/inductor-x (imported there a
   ``get_current_raw_stream`` from this package (``NewNPUDeviceOpOverrides``),
 * registers the Dynamo device interface (``NewNpuInterface``),
 * applies the lowering policy and decomposition edits, and
-* registers the fused-attention FX pattern.
+* registers the fused-attention FX pattern and the operators of a windowed decoder layer.
 
 After that ``torch.compile(fn)`` on CUDA tensors emits no Triton: every fused group becomes
 an instantiation of a hand-written CUDA template, compiled once and called through the C ABI.
@@ -143,6 +143,7 @@ def register():
     _register_b200_inductor_fallbacks()
     _register_b200_inductor_decompositions()
     from . import fusion_attention_graph
+    from . import window_ops  # noqa: F401  (operators of a windowed decoder layer)
 
     fusion_attention_graph.register_fx_pass()
     _registered = True

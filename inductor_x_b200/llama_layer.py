@@ -1,7 +1,10 @@
 """The Llama-style decoder layer of benchmark configuration 5, written as the plain PyTorch
 graph a user would hand to ``torch.compile``: RMSNorm, QKV projections, rotary embedding,
 causal attention, output projection, residual, RMSNorm, SwiGLU feed-forward, residual.
-It exists so that tests and the benchmark compile the same graph; it is not a model zoo."""
+It exists so that tests and the benchmark compile the same graph; it is not a model zoo.
+
+The attention half of a layer with a sliding window, shared key heads and positions with several axes stands beside it: for
+training (``window_attention_half``) and for serving over a cache with 8-bit projections (``window_attention_step``)."""
 from __future__ import annotations
 
 import math
@@ -37,3 +40,50 @@ def decoder_layer(x, w, cos, sin, heads: int = 32, eps: float = 1e-6):
     h2 = rms_norm(h, w["norm2"], eps)
     ff = F.linear(F.silu(F.linear(h2, w["w_gate"])) * F.linear(h2, w["w_up"]), w["w_down"])
     return h + ff
+
+
+def window_attention_half(x, w, positions, *, heads: int, kv_heads: int, sections, window: int, sinks: int = 0,
+                          lengths=None, base: float = 10000.0, eps: float = 1e-6):
+    """``x`` plus the attention of its norm: RMSNorm, projections, rotary positions, windowed attention, output projection.
+    x [B, S, hidden]; w: dict with norm1, wq, wk, wv, wo; positions [axes, B, S]; lengths int32 [B] of a padded batch.
+    Differentiable in x and w."""
+    from . import window_ops  # noqa: F401  (registers the operators)
+
+    B, S, Hd = x.shape
+    D = w["wq"].shape[0] // heads
+    h = rms_norm(x, w["norm1"], eps)
+    split = lambda t, n: t.view(B, S, n, D).transpose(1, 2)  # noqa: E731
+    q, k, v = split(F.linear(h, w["wq"]), heads), split(F.linear(h, w["wk"]), kv_heads), split(F.linear(h, w["wv"]), kv_heads)
+    q, k = torch.ops.b200_graph.b200_axial_rotary(q, k, positions, sections, base)
+    a, _ = torch.ops.b200_graph.b200_window_attention(q, k, v, 1.0 / math.sqrt(D), window, sinks, lengths, lengths)
+    return x + F.linear(a.transpose(1, 2).reshape(B, S, heads * D), w["wo"])
+
+
+def quantise_rows(weight: torch.Tensor):
+    """A projection's weight [out, in] in 8 bits with a scale for each row, as ``window_attention_step`` takes it."""
+    scales = weight.float().abs().amax(1, keepdim=True).clamp(min=1e-12) / 448.0
+    return (weight.float() / scales).to(torch.float8_e4m3fn), scales
+
+
+def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, *, heads: int, kv_heads: int, sections,
+                          window: int, sinks: int = 0, base: float = 10000.0, eps: float = 1e-6):
+    """One token of each sequence: the residual is added and normalised to 8 bits, projected, turned and written to the
+    cache at ``lengths`` (int32 [B], which it then advances), and attends to what its window leaves of the cache.
+    x, residual [B, hidden]; w: dict with norm1 and, from :func:`quantise_rows`, wqkv, and wo; positions [axes, B, 1];
+    cache_k, cache_v [B, kv_heads, capacity, D].  Returns the output projection and the new residual."""
+    from . import ops
+
+    B = x.shape[0]
+    D = cache_k.shape[3]
+    h8, scales, residual = ops.rmsnorm_quantised(x, w["norm1"], eps, residual=residual, return_residual=True)
+    w8, w_scales = w["wqkv"]
+    # (a row and a column scale: a plain library product)
+    qkv = torch._scaled_mm(h8, w8.t(), scale_a=scales[:, None], scale_b=w_scales.t(), out_dtype=x.dtype)
+    q, k, v = (t.view(B, 1, -1, D).transpose(1, 2) for t in qkv.split([heads * D, kv_heads * D, kv_heads * D], dim=1))
+    q, k = ops.axial_rotary(q, k, positions, sections, base=base)
+    rows = torch.arange(B, device=x.device)
+    cache_k[rows, :, lengths.long()] = k[:, :, 0]
+    cache_v[rows, :, lengths.long()] = v[:, :, 0]
+    lengths += 1
+    a = ops.window_attention(q, cache_k, cache_v, 1.0 / math.sqrt(D), window=window, sinks=sinks, kv_lengths=lengths)
+    return F.linear(a.view(B, heads * D), w["wo"]), residual

@@ -527,6 +527,11 @@ def _rotary_plan(sections: tuple, base: float, ladder: str, frequencies: Optiona
     return (pairs, len(sections), c_sections, c_frequencies, ctypes.addressof(c_sections), ctypes.addressof(c_frequencies))
 
 
+def _rotary_result(t: torch.Tensor) -> torch.Tensor:
+    """In the memory order of the input; an expanded input's is a dense tensor of its own."""
+    return torch.empty_like(t) if all(t.stride()) else t.new_empty(t.shape)
+
+
 def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inverse):
     if pairing not in PAIRINGS or ladder not in LADDERS:
         raise ValueError(f"pairing must be one of {PAIRINGS}, ladder one of {LADDERS}")
@@ -549,9 +554,7 @@ def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inver
         raise ValueError("the head dimension must be contiguous")
     _one_device(q, k, positions)
     at = positions.stride() if positions.dim() == 3 else (positions.stride(0), 0, positions.stride(1))
-    # (an expanded input's result is a dense tensor of its own)
-    new = lambda t: torch.empty_like(t) if all(t.stride()) else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    q_out, k_out = new(q), None if k is None else new(k)
+    q_out, k_out = _rotary_result(q), None if k is None else _rotary_result(k)
     strides = lambda t: _I64x3(*t.stride()[:3]) if t is not None else None  # noqa: E731
     if q.numel() or (k is not None and k.numel()):
         with torch.cuda.device(q.device):
