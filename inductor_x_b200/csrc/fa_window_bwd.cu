@@ -29,6 +29,9 @@ constexpr int kThreads = 128 + kWorkers;  // producer, issuer and scheduler; the
 // Registers: the block starts with kRegsLaunch a thread (all that 12 warps can have)
 constexpr int kRegsLaunch = 168, kRegsIssue = 80, kRegsWork = 208;
 static_assert(kRegsIssue + NG * kRegsWork <= (1 + NG) * kRegsLaunch, "setmaxnreg draws on the block's own registers");
+// the dQ kernel has a warpgroup more, which stores the results
+constexpr int kDqThreads = kThreads + 128, kDqRegsLaunch = 128, kDqRegsIssue = 80, kDqRegsWork = 168, kDqRegsStore = 96;
+static_assert(kDqRegsIssue + NG * kDqRegsWork + kDqRegsStore <= (2 + NG) * kDqRegsLaunch, "setmaxnreg draws on the block's own registers");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kCol0 = 0, kCol1 = 128, kCol2 = 256, kCol3 = 384;
 constexpr int kKeyStages = 3;  // of K in the dQ kernel
@@ -603,8 +606,10 @@ __global__ void __launch_bounds__(256) window_sinks_kernel(const BwdParams p) {
 
 // ------------------------------------------------------------------------------ dQ
 // TMEM columns: [0,128) S, [128,256) and [256,384) dP then dS of the steps in turn, [384,512) dQ.
+// The results leave through four warps of their own, so that the element-wise warps go on to the next item's scores: those and
+// the statistics, which the producer reads ahead, took 7100 of the 24700 cycles of an item of nine steps before.
 template <bool IS_BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kDqThreads, 1)
     window_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const BwdParams p) {
   extern __shared__ unsigned char smem_raw[];
@@ -618,6 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(16) uint4 next_answer[2];
   __shared__ __align__(8) uint64_t next_wanted, next_full[2], next_taken[2], q_full, q_empty, do_full, do_empty, k_full[kKeyStages],
       k_empty[kKeyStages], v_full[kStages], v_empty[kStages], raw_full, s_full, s_read, dp_full[2], ds_full[2], acc_done, acc_empty, drained;
+  // of the query tile: -lse in log2 units (-inf where nothing is seen: P = 0) and -delta
+  __shared__ float nlse_s[BM], ndelta_s[BM];
   __shared__ uint32_t tmem_base_slot;
   __shared__ volatile int failed;
 
@@ -654,12 +661,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&next_wanted, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&next_full[s], 1);
-      mbar_init(&next_taken[s], 2 + kWorkers / 32);  // producer, issuer and element-wise warps
+      mbar_init(&next_taken[s], 2 + kWorkers / 32 + 4);  // producer, issuer, element-wise and storing warps
       mbar_init(&dp_full[s], 1);
       mbar_init(&ds_full[s], kWorkers / 32);
     }
-    mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1);
+    mbar_init(&q_full, 2);                   // the copy and the statistics
+    mbar_init(&q_empty, 1 + kWorkers / 32);  // the last product, and those who have read the statistics
     mbar_init(&do_full, 1);
     mbar_init(&do_empty, 1);
     for (int s = 0; s < kKeyStages; ++s) {
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s_full, 1);
     mbar_init(&s_read, kWorkers / 32);
     mbar_init(&acc_done, 1);
-    mbar_init(&acc_empty, kWorkers / 32);
+    mbar_init(&acc_empty, 4);
     mbar_init(&drained, 1);
     failed = 0;
     mbar_init_fence();
@@ -689,19 +696,37 @@ __global__ void __launch_bounds__(kThreads, 1)
   int q_loads = 0, do_loads = 0, k_loads = 0, v_loads = 0, raw_loads = 0;  // producer: what it has asked for
   bool raw_pending = false;
   int asked = 0;                                                           // scheduler: the same
-  if (warp < 4) tc::regs_dec<kRegsIssue>();
+  if (warp < 4) tc::regs_dec<kDqRegsIssue>();
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     bool ok = true;
     for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
       const Item w = item_of(index);
+      float lse_r[4], delta_r[4];
       if (w.n_kv > 0) {
+        // (read before the wait, so that nothing waits for the reads)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int qi = w.qt0 + e * 32 + lane;
+          const long long at = ((long long)w.b * p.H + w.h) * p.Sq + qi;
+          const bool live = qi < w.n.q && w.n.off + qi >= 0;  // (any other sees nothing, and may hold anything)
+          lse_r[e] = live ? p.lse[at] * -kLog2e : -INFINITY;
+          delta_r[e] = live ? -p.delta[at] : 0.f;
+          if (lse_r[e] == INFINITY) lse_r[e] = -INFINITY;     // (and so does a row whose log-sum-exp is -inf)
+        }
         if (q_loads > 0) ok = __all_sync(kFull, mbar_wait(&q_empty, (q_loads - 1) & 1, &failed));
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&q_full, kTileBytes);
           load_tile(q_smem, &map_q, &q_full, w.qt0, w.h, w.b);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          nlse_s[e * 32 + lane] = lse_r[e];
+          ndelta_s[e * 32 + lane] = delta_r[e];
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&q_full);
         ++q_loads;
       }
       for (int x = 0; x < w.n_kv && ok; ++x) {
@@ -815,9 +840,43 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 2) {
     asked = pending.run(lane, &failed);
+  } else if (warp >= 4 + 4 * NG) {
+    // ------------------------------------------------------------------ results
+    tc::regs_dec<kDqRegsStore>();
+    const int quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t acc_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + kCol3;
+    bool ok = true;
+    int items = 0;
+    for (int n = 0, index = blockIdx.x; index >= 0 && ok; ++n) {
+      const Item w = item_of(index);
+      const int qi = w.qt0 + row;
+      // a row that sees nothing, whatever its products hold (its log-sum-exp says so where its position does not)
+      bool some = qi < w.n.q && w.n.off + qi >= 0;
+      if (some) some = p.lse[((long long)w.b * p.H + w.h) * p.Sq + qi] != -INFINITY;
+      unsigned char* dq_row = reinterpret_cast<unsigned char*>(p.dq.ptr) +
+                              2 * ((long long)w.b * p.dq.sb + (long long)w.h * p.dq.sh + (long long)qi * p.dq.ss);
+      if (w.n_kv > 0) {
+        ok = __all_sync(kFull, mbar_wait(&acc_done, items & 1, &failed));
+        if (!ok) break;
+        tc::fence_after_sync();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) store_cols<IS_BF16>(acc_addr + GC * g, dq_row + 2 * GC * g, p.scale, qi < p.Sq && some, p.dq.wide);
+        tc::fence_before_sync();
+        warp_arrive(&acc_empty, lane);
+        ++items;
+      }
+      if (qi < p.Sq && !(some && w.n_kv > 0)) {
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int e = 0; e < HD / 8; ++e) reinterpret_cast<uint4*>(dq_row)[e] = z;
+      }
+      __syncwarp();
+      index = pending.take_next(n, lane, ok, &failed);
+    }
+    if (!ok && lane == 0) failed = 1;
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ element-wise work
-    tc::regs_inc<kRegsWork>();
+    tc::regs_inc<kDqRegsWork>();
     const int g = (warp - 4) >> 2;  // group: key columns [GC g, GC g + GC) of a tile
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
@@ -831,12 +890,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item w = item_of(index);
       const int qi = w.qt0 + row;
       const int at = qi < w.n.q ? w.n.off + qi : -1;  // (below 0: sees nothing)
-      const long long stat_at = ((long long)w.b * p.H + w.h) * p.Sq + qi;
-      const float lse = at >= 0 ? p.lse[stat_at] : -INFINITY;
-      const bool some = lse != -INFINITY;
-      const float dl = some ? p.delta[stat_at] : 0.f;
-      const float nl = some ? -lse * kLog2e : -INFINITY;
-      const float2 nl2 = make_float2(nl, nl), ndl2 = make_float2(-dl, -dl);
+      float2 nl2, ndl2;
+      if (w.n_kv > 0) {
+        ok = __all_sync(kFull, mbar_wait(&q_full, items & 1, &failed));
+        if (!ok) break;
+        nl2 = make_float2(nlse_s[row], nlse_s[row]);
+        ndl2 = make_float2(ndelta_s[row], ndelta_s[row]);
+        warp_arrive(&q_empty, lane);
+        ++items;
+      }
       const int at_first = w.n.off + w.qt0, at_last = at_first + BM - 1;
       for (int x = 0; x < w.n_kv; ++x, ++step) {
         if (!__all_sync(kFull, mbar_wait(&s_full, step & 1, &failed))) {
@@ -894,28 +956,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_arrive(&ds_full[step & 1], lane);
       }
 
-      if (ok && w.n_kv > 0) ok = mbar_wait(&acc_done, items & 1, &failed);
-      ok = __all_sync(kFull, ok);
-      if (ok) {
-        tc::fence_after_sync();
-        unsigned char* dq_row = reinterpret_cast<unsigned char*>(p.dq.ptr) +
-                                2 * ((long long)w.b * p.dq.sb + (long long)w.h * p.dq.sh + (long long)qi * p.dq.ss) + 2 * GC * g;
-        if (w.n_kv > 0) {
-          store_cols<IS_BF16>(lane_addr + kCol3 + GC * g, dq_row, p.scale, qi < p.Sq && some, p.dq.wide);
-          tc::fence_before_sync();
-          warp_arrive(&acc_empty, lane);
-          ++items;
-        }
-        if (qi < p.Sq && !(some && w.n_kv > 0)) {
-          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-          for (int e = 0; e < GC / 8; ++e) reinterpret_cast<uint4*>(dq_row)[e] = z;
-        }
-      }
       __syncwarp();
       index = pending.take_next(n, lane, ok, &failed);
     }
-    if (!ok) failed = 1;
+    if (!ok && lane == 0) failed = 1;
   }
 
   tc::fence_before_sync();
@@ -941,12 +985,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // The opt-ins of a kernel on the current device, asked for once: a property of (kernel, device).
 template <class K>
-int opt_in(K kern, std::atomic<bool>& done, size_t smem) {
+int opt_in(K kern, std::atomic<bool>& done, size_t smem, int regs) {
   if (!done.load(std::memory_order_acquire)) {
     cudaFuncAttributes at;  // (as in fa_fwd.cu: setmaxnreg waits for registers the block has to own)
     cudaError_t e = cudaFuncGetAttributes(&at, kern);
     if (e != cudaSuccess) return ixb_host::cuda_status(e);
-    if (at.numRegs != kRegsLaunch) return IXB_ERR_UNSUPPORTED;
+    if (at.numRegs != regs) return IXB_ERR_UNSUPPORTED;
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return ixb_host::cuda_status(e);
     done.store(true, std::memory_order_release);
@@ -1027,8 +1071,8 @@ extern "C" int ixb_window_attention_bwd(int dtype, const void* q, const void* k,
   static std::atomic<bool> configured[2][2][64];
   int devid = 0;
   cudaGetDevice(&devid);
-  if (int st = opt_in(kern_dkv, configured[0][is_bf16][devid & 63], kDkvSmem)) return st;
-  if (int st = opt_in(kern_dq, configured[1][is_bf16][devid & 63], kDqSmem)) return st;
+  if (int st = opt_in(kern_dkv, configured[0][is_bf16][devid & 63], kDkvSmem, kRegsLaunch)) return st;
+  if (int st = opt_in(kern_dq, configured[1][is_bf16][devid & 63], kDqSmem, kDqRegsLaunch)) return st;
   const cudaStream_t cs = (cudaStream_t)stream;
   kern_delta<<<(unsigned)delta_blocks, 256, 0, cs>>>(
       static_cast<const unsigned char*>(o), static_cast<const unsigned char*>(dout), delta, H, Sq, (Sq + 63) / 64,
@@ -1038,6 +1082,6 @@ extern "C" int ixb_window_attention_bwd(int dtype, const void* q, const void* k,
     const long long pieces = (long long)B * HK * sinks * 2 * (HD / 4);
     kern_sinks<<<(unsigned)((pieces + 255) / 256), 256, 0, cs>>>(p);
   }
-  kern_dq<<<(unsigned)dq_items, kThreads, kDqSmem, cs>>>(mq, mk, mv, mdo, p);
+  kern_dq<<<(unsigned)dq_items, kDqThreads, kDqSmem, cs>>>(mq, mk, mv, mdo, p);
   return ixb_host::cuda_status(cudaGetLastError());
 }
