@@ -146,7 +146,7 @@ int ixb_rmsnorm(int dtype, const void* x, const void* res, const void* w, void* 
  * y = h * rsqrt(mean(h*h) + eps) * w in fp32; scales = max|y| / 448 over the row (group 0: scales[rows]) or
  * over each 128 of its values (group 128: scales[rows, ceil(cols / 128)], the last over what is left);
  * q[rows, cols] = e4m3(y / scale), to the nearest.  Where scale is 0 so is q; a NaN or an infinity of y
- * makes its scale and what it covers NaN.  res and h_out may be null.  No counterpart in the reference: its norms
+ * makes its scale and what it covers NaN.  res and h_out may be null; rows below 2^31, cols at most 2^20.  No counterpart in the reference: its norms
  * leave 16 bits (inductor_x/lowering.py:217-233). */
 int ixb_rmsnorm_quantised(int dtype, const void* x, const void* res, const void* w, void* q,
                           float* scales, void* h_out, int64_t rows, int64_t cols, int32_t group,
@@ -287,23 +287,19 @@ int ixb_fa_bwd_scratch(int dtype, const void* q, const void* k, const void* v, c
  * values outside [0, Sq] and [0, Sk] count as the nearest of those).  Query i of sequence b stands at position
  * p = kv_lengths[b] - q_lengths[b] + i and sees key j when j <= p and (j > p - window or j < sinks) and
  * j < kv_lengths[b]; a query that sees nothing, and any at or behind q_lengths[b], gets o = 0 and lse = -inf.
- * lse[B,H,Sq] may be null.  window >= 1, 0 <= sinks <= 128, Sk >= 1, scale > 0 and finite.  `scratch` (16-byte
- * aligned, contents lost) of ixb_window_attention_scratch_bytes bytes, which may be 0.  `status` as in
+ * lse[B,H,Sq] may be null.  window >= 1, 0 <= sinks <= 128, Sk >= 1, scale > 0 and finite.  `status` as in
  * ixb_fa_fwd.  The reference passes such bounds to the vendor kernel as pre_tockens / next_tockens
  * (inductor_x/npu_fusion_attention_graph.py:13-18). */
-size_t ixb_window_attention_scratch_bytes(int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk,
-                                          int32_t window, int32_t sinks);
 int ixb_window_attention(int dtype, const void* q, const void* k, const void* v, void* o,
-                         float* lse, void* scratch, size_t scratch_bytes, int32_t B, int32_t H,
-                         int32_t HK, int32_t Sq, int32_t Sk, int32_t D, const int64_t* q_strides,
-                         const int64_t* k_strides, const int64_t* v_strides,
+                         float* lse, int32_t B, int32_t H, int32_t HK, int32_t Sq, int32_t Sk,
+                         int32_t D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                          const int64_t* o_strides, const int32_t* q_lengths,
                          const int32_t* kv_lengths, float scale, int32_t window, int32_t sinks,
                          int32_t* status, ixb_stream stream);
 
 /* Gradients of ixb_window_attention from its output `o` and log-sum-exp `lse`; dk and dv are summed over
  * the query heads that share a key head.  Every element of dq, dk and dv is written: zeros where nothing
- * was seen.  No atomics: the same bits every time.  `scratch` of ixb_window_attention_bwd_scratch_bytes
+ * was seen (B, H > 0; Sq, Sk >= 1).  No atomics: the same bits every time.  `scratch` of ixb_window_attention_bwd_scratch_bytes
  * bytes, 16-byte aligned, contents lost. */
 size_t ixb_window_attention_bwd_scratch_bytes(int32_t B, int32_t H, int32_t HK, int32_t Sq,
                                               int32_t Sk, int32_t window, int32_t sinks);
@@ -324,7 +320,7 @@ int ixb_window_attention_bwd(int dtype, const void* q, const void* k, const void
  * order, at most 128 together and 2 * pairs <= D; frequencies[pairs] (host memory): radians a position.  Pair i of
  * a head is turned by positions[axis(i), b, s] * frequencies[i], the angle formed in 64 bits; pair i is
  * (i, pairs + i), or (2i, 2i + 1) with neighbours != 0; what lies behind the pairs is copied.  inverse != 0 turns the
- * other way: the gradient.  positions I64 or I32 with the strides of its three axes in elements.  The reference has
+ * other way: the gradient.  positions I64 or I32 with the strides of its three axes in elements; B * S at most 2^30.  The reference has
  * rotary embeddings as pointwise graphs only (inductor_x/lowering.py:45-88). */
 int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int64_t* q_strides,
                      const int64_t* q_out_strides, int32_t heads, const void* k, void* k_out,

@@ -83,6 +83,13 @@ template <class T> struct Pairs {
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) v[e] = mul2(mul2(v[e], make_float2(r, r)), g.v[e]);
   }
+  __device__ __forceinline__ void keep(uint32_t lives) {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      if (!(lives >> e & 1u)) v[e / 2].x = 0.f;
+      if (!(lives >> (e + 1) & 1u)) v[e / 2].y = 0.f;
+    }
+  }
   __device__ __forceinline__ uint32_t bits(int e) const { return __float_as_uint(e & 1 ? v[e / 2].y : v[e / 2].x); }
   __device__ __forceinline__ uint32_t largest(uint32_t m = 0) const {
 #pragma unroll
@@ -169,12 +176,12 @@ __global__ void __launch_bounds__(W < 8 ? 256 : W * 32) norm_quantised_kernel(co
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     f[u].scale(r, raw[u]);
-    // (behind the row there are zeros, times what the row's values are multiplied with: a number, or all of the row is NaN)
+    const uint32_t mine = col(u) < cols ? f[u].largest() : 0u;  // (behind the row there are zeros, but r may be infinite)
     if (p.group == 0) {
-      top = f[u].largest(top);
+      top = max(top, mine);
       continue;
     }
-    const uint32_t m = group_max<kLanes>(f[u].largest());
+    const uint32_t m = group_max<kLanes>(mine);
     if (lane % kLanes == 0 && col(u) < cols) p.scales[row * ((p.cols + kGroup - 1) / kGroup) + col(u) / kGroup] = scale_of(m);
     put(u, m);
   }
@@ -263,8 +270,7 @@ __global__ void __launch_bounds__(W < 8 ? 256 : W * 32, W <= 8 ? 4 : W == 16 ? 2
     float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      // (a vector's elements of other rows count as zero: their norm is 0 times what the row's values are multiplied
-      // with, which is a number or makes all of the row NaN)
+      // (a vector's elements of other rows count as zero)
       if (lives[u] != kAll) {
         raw[u] = kept<E>(raw[u], lives[u]);
         if (p.res != nullptr) more[u] = kept<E>(more[u], lives[u]);
@@ -305,6 +311,7 @@ __global__ void __launch_bounds__(W < 8 ? 256 : W * 32, W <= 8 ? 4 : W == 16 ? 2
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       f[u].scale(r, w[u]);
+      if (lives[u] != kAll) f[u].keep(lives[u]);  // (r may be infinite)
       if (p.group == 0) {
         top = f[u].largest(top);
         continue;

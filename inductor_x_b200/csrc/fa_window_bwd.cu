@@ -998,15 +998,16 @@ int opt_in(K kern, std::atomic<bool>& done, size_t smem, int regs) {
   return IXB_OK;
 }
 
-// Items that the queries behind the first key tile's window are cut into, of about as many steps as another item has
-// (at least 8); none where there are no such queries or no first tokens.
+// Items that the queries behind the first key tile's window are cut into, of as many steps as another item has, or as
+// make 128 of them (each leaves sinks x 1 KB of sums); none where there are no such queries or no first tokens.
 int sink_chunks(int H, int HK, int Sq, int Sk, int window, int sinks) {
   if (sinks == 0 || window >= Sk) return 0;
   const long long share = H / HK, q_tiles = ((long long)Sq + BM - 1) / BM;
   const long long behind = ((long long)Sk - window + BM - 1) / BM + 1;
   const long long all = share * (behind < q_tiles ? behind : q_tiles);
   const long long each = share * (((long long)window + 2 * BM - 2) / BM + 1);
-  return (int)((all + (each > 8 ? each : 8) - 1) / (each > 8 ? each : 8));
+  const long long items = (all + each - 1) / each;
+  return (int)(items < 128 ? items : 128);
 }
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t delta_bytes(int B, int H, int Sq) { return round16((size_t)B * H * Sq * sizeof(float)); }

@@ -156,17 +156,16 @@ decltype(&ixb_fa_bwd_scratch) entry_fa_bwd;
 decltype(&ixb_rmsnorm_quantised) entry_rmsnorm_quantised;
 decltype(&ixb_axial_rotary) entry_rotary;
 decltype(&ixb_window_attention) entry_window;
-decltype(&ixb_window_attention_scratch_bytes) entry_window_room;
 decltype(&ixb_window_attention_bwd) entry_window_bwd;
 decltype(&ixb_window_attention_bwd_scratch_bytes) entry_window_bwd_room;
 
-// bind_library(rmsnorm, fa_fwd, fa_bwd_scratch_bytes, fa_bwd_scratch, rmsnorm_quantised, axial_rotary, window_attention and its
-// scratch_bytes, window_attention_bwd and its scratch_bytes): addresses of the C entries
+// bind_library(rmsnorm, fa_fwd, fa_bwd_scratch_bytes, fa_bwd_scratch, rmsnorm_quantised, axial_rotary, window_attention,
+// window_attention_bwd and its scratch_bytes): addresses of the C entries
 PyObject* bind_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr int kEntries = 10;
+  constexpr int kEntries = 9;
   void* p[kEntries];
   if (n != kEntries) {
-    PyErr_SetString(PyExc_TypeError, "bind_library takes ten addresses");
+    PyErr_SetString(PyExc_TypeError, "bind_library takes nine addresses");
     return nullptr;
   }
   for (int i = 0; i < kEntries; ++i) {
@@ -180,9 +179,8 @@ PyObject* bind_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   entry_rmsnorm_quantised = reinterpret_cast<decltype(entry_rmsnorm_quantised)>(p[4]);
   entry_rotary = reinterpret_cast<decltype(entry_rotary)>(p[5]);
   entry_window = reinterpret_cast<decltype(entry_window)>(p[6]);
-  entry_window_room = reinterpret_cast<decltype(entry_window_room)>(p[7]);
-  entry_window_bwd = reinterpret_cast<decltype(entry_window_bwd)>(p[8]);
-  entry_window_bwd_room = reinterpret_cast<decltype(entry_window_bwd_room)>(p[9]);
+  entry_window_bwd = reinterpret_cast<decltype(entry_window_bwd)>(p[7]);
+  entry_window_bwd_room = reinterpret_cast<decltype(entry_window_bwd_room)>(p[8]);
   Py_RETURN_NONE;
 }
 
@@ -485,17 +483,14 @@ PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!c.ok) Py_RETURN_NONE;
     at::Tensor out = at::empty({c.B, c.H, c.Sq, 128}, c.q->options()), lse;
     if (args[8] == Py_True) lse = at::empty({c.B, c.H, c.Sq}, c.q->options().dtype(at::kFloat));
-    const size_t room = entry_window_room(c.B, c.H, c.HK, c.Sq, c.Sk, c.window, c.sinks);
     const c10::OptionalDeviceGuard device(c.q->device());
-    c10::DataPtr scratch;  // memory as it is (see fused_attention_backward)
-    if (room) scratch = c10::GetAllocator(c10::kCUDA)->allocate(room);
     const OperandStrides qs(*c.q), ks(*c.k), vs(*c.v), os(out);
     const ixb_stream stream = stream_of(*c.q);
     const float scale = (float)PyFloat_AS_DOUBLE(args[3]);
     int st;
     Py_BEGIN_ALLOW_THREADS
     st = entry_window(dtype_code(*c.q), c.q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(), out.data_ptr(),
-                      lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, scratch.get(), room, c.B, c.H, c.HK, c.Sq, c.Sk, 128, qs.v, ks.v,
+                      lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, c.B, c.H, c.HK, c.Sq, c.Sk, 128, qs.v, ks.v,
                       vs.v, os.v, WindowCall::ptr(c.q_lengths), WindowCall::ptr(c.kv_lengths), scale, c.window, c.sinks, nullptr, stream);
     Py_END_ALLOW_THREADS
     if (st != 0) return PyLong_FromLong(st);
@@ -517,6 +512,7 @@ PyObject* window_attention_backward(PyObject*, PyObject* const* args, Py_ssize_t
     const OperandStrides qs(*c.q), ks(*c.k), vs(*c.v), os(*o), gs(*go);
     for (int i = 0; i < 3; ++i)
       if (gs.v[i] <= 0 || gs.v[i] % 8 != 0) Py_RETURN_NONE;
+    if ((reinterpret_cast<uintptr_t>(go->data_ptr()) & 15u) != 0) Py_RETURN_NONE;
     if (lse->dim() != 3 || lse->size(0) != c.B || lse->size(1) != c.H || lse->size(2) != c.Sq || lse->scalar_type() != at::kFloat ||
         lse->device() != c.q->device() || !lse->is_contiguous())
       Py_RETURN_NONE;
@@ -524,7 +520,7 @@ PyObject* window_attention_backward(PyObject*, PyObject* const* args, Py_ssize_t
                dv = at::empty({c.B, c.HK, c.Sk, 128}, c.q->options());
     const size_t room = entry_window_bwd_room(c.B, c.H, c.HK, c.Sq, c.Sk, c.window, c.sinks);
     const c10::OptionalDeviceGuard device(c.q->device());
-    const c10::DataPtr scratch = c10::GetAllocator(c10::kCUDA)->allocate(room);
+    const c10::DataPtr scratch = c10::GetAllocator(c10::kCUDA)->allocate(room);  // memory as it is (see fused_attention_backward)
     const OperandStrides dqs(dq), dks(dk), dvs(dv);
     const ixb_stream stream = stream_of(*c.q);
     const float scale = (float)PyFloat_AS_DOUBLE(args[6]);

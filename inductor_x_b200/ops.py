@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -405,6 +406,7 @@ def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
         raise ValueError("the head dimension must be 128")
     if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v, *more)):
         raise ValueError("q, k, v (and out, dout) must share dtype float16 or bfloat16")
+    window, sinks = operator.index(window), operator.index(sinks)
     if not 1 <= window:
         raise ValueError("window must be at least 1")
     if not 0 <= sinks <= 128:
@@ -417,7 +419,7 @@ def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
             raise ValueError("the head dimension must be contiguous")
     _one_device(q, k, v, q_lengths, kv_lengths, *more)
     most = 2 ** 31 - 1
-    return (min(int(window), most), int(sinks), q_lengths.contiguous() if q_lengths is not None else None,
+    return (min(window, most), sinks, q_lengths.contiguous() if q_lengths is not None else None,
             kv_lengths.contiguous() if kv_lengths is not None else None)
 
 
@@ -448,13 +450,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
         out.zero_()
         return (out, lse.fill_(float("-inf"))) if return_lse else out
     status = torch.zeros(1, dtype=torch.int32, device=q.device) if check else None
-    lib = rt.load()
-    room = lib.ixb_window_attention_scratch_bytes(B, H, HK, Sq, Sk, window, sinks)
-    scratch = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
     with torch.cuda.device(q.device):
-        rt.check("ixb_window_attention", lib.ixb_window_attention(
-            rt.DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rt.ptr(lse), rt.ptr(scratch),
-            room, B, H, HK, Sq, Sk, D, _operand_strides(q), _operand_strides(k), _operand_strides(v), _operand_strides(out),
+        rt.check("ixb_window_attention", rt.load().ixb_window_attention(
+            rt.DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rt.ptr(lse), B, H, HK, Sq, Sk, D, _operand_strides(q), _operand_strides(k), _operand_strides(v), _operand_strides(out),
             rt.ptr(q_lengths), rt.ptr(kv_lengths), float(scale), window, sinks, rt.ptr(status), rt.raw_stream(q.device)))
     if status is not None and int(status.item()) != 0:
         raise RuntimeError("ixb_window_attention: an internal pipeline wait gave up; output is undefined")
@@ -483,13 +481,14 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError("lse must be float32 [B, H, Sq]")
     _one_device(q, out, lse, dout)
     lse = lse.contiguous()
-    if dout.numel() and (dout.stride(3) != 1 or any(st <= 0 or st % 8 for st in _operand_strides(dout))):
-        dout = dout.contiguous()
+    if dout.numel() and (dout.stride(3) != 1 or any(st <= 0 or st % 8 for st in _operand_strides(dout))
+                         or dout.data_ptr() % 16):
+        dout = dout.clone(memory_format=torch.contiguous_format)
     if out.numel() and out.stride(3) != 1:
         raise ValueError("the head dimension must be contiguous")
     dq = torch.empty((B, H, Sq, D), dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty((B, HK, Sk, D), dtype=q.dtype, device=q.device) for _ in range(2))
-    if Sq == 0 or Sk == 0:
+    if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     status = torch.zeros(1, dtype=torch.int32, device=q.device) if check else None
     lib = rt.load()

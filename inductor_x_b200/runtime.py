@@ -110,8 +110,7 @@ _SIGNATURES = {
     "ixb_fa_bwd_scratch": (c_int, [c_int] + [c_void_p] * 11 + [c_size_t] + [c_int32] * 5 + [POINTER(c_int64)] * 8 +
                            [c_float, c_int, c_void_p, c_void_p]),
     "ixb_rmsnorm_quantised": (c_int, [c_int] + [c_void_p] * 6 + [c_int64] * 2 + [c_int32, c_float, c_void_p]),
-    "ixb_window_attention_scratch_bytes": (c_size_t, [c_int32] * 7),
-    "ixb_window_attention": (c_int, [c_int] + [c_void_p] * 6 + [c_size_t] + [c_int32] * 6 + [POINTER(c_int64)] * 4 +
+    "ixb_window_attention": (c_int, [c_int] + [c_void_p] * 5 + [c_int32] * 6 + [POINTER(c_int64)] * 4 +
                              [c_void_p] * 2 + [c_float, c_int32, c_int32, c_void_p, c_void_p]),
     "ixb_window_attention_bwd_scratch_bytes": (c_size_t, [c_int32] * 7),
     "ixb_window_attention_bwd": (c_int, [c_int] + [c_void_p] * 10 + [c_size_t] + [c_int32] * 6 + [POINTER(c_int64)] * 8 +
@@ -149,8 +148,7 @@ def load() -> ctypes.CDLL:
 
     _ixb_host.bind_library(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
         "ixb_rmsnorm", "ixb_fa_fwd", "ixb_fa_bwd_scratch_bytes", "ixb_fa_bwd_scratch", "ixb_rmsnorm_quantised", "ixb_axial_rotary",
-        "ixb_window_attention", "ixb_window_attention_scratch_bytes", "ixb_window_attention_bwd",
-        "ixb_window_attention_bwd_scratch_bytes")))
+        "ixb_window_attention", "ixb_window_attention_bwd", "ixb_window_attention_bwd_scratch_bytes")))
     _lib = lib
     return lib
 

@@ -79,6 +79,15 @@ def test_zeros_tiny_and_huge_rows(cuda, cols):
         assert bool((q.float().abs().max() >= 400)) and bool((s > 0).all())
 
 
+@pytest.mark.parametrize("cols", [72, 77, 260, 1537])
+def test_rows_whose_root_is_infinite(cuda, cols):
+    """Without eps the squares of tiny values are zero: what lies beside a row's end must not come in."""
+    x = torch.full((9, cols), 1e-30, device=cuda)
+    for group in (0, 128):
+        q, s = ops.rmsnorm_quantised(x, torch.ones(cols, device=cuda), 0.0, group=group)
+        assert bool(torch.isinf(s).all()) and bool(torch.isnan(q.float()).all())
+
+
 def test_values_that_are_not_finite(cuda):
     x = torch.randn(4, 512, device=cuda)
     x[1, 200] = math.nan

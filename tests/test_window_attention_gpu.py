@@ -163,6 +163,53 @@ def test_no_keys_and_no_queries(cuda):
     assert ops.window_attention(empty, kk[:0], kk[:0], 0.1, window=4).shape == empty.shape
 
 
+def test_no_heads(cuda):
+    q, k = torch.empty(2, 0, 3, 128, device=cuda).half(), torch.randn(2, 2, 5, 128, device=cuda).half()
+    out, lse = ops.window_attention(q, k, k, 0.1, window=4, return_lse=True)
+    dq, dk, dv = ops.window_attention_backward(q, k, k, out, lse, out, 0.1, window=4)
+    assert out.shape == q.shape and dq.shape == q.shape and not dk.any() and not dv.any()
+
+
+def test_gradients_off_a_boundary_are_taken(cuda):
+    """An incoming gradient may start and step anywhere."""
+    q, k, v, g, _, _ = make(cuda, torch.bfloat16, 2, 2, 1, 70, 90, seed=4)
+    out, lse = ops.window_attention(q, k, v, 0.1, window=30, return_lse=True)
+    expected = ops.window_attention_backward(q, k, v, out, lse, g, 0.1, window=30)
+    off = torch.empty(g.numel() + 1, device=cuda, dtype=g.dtype)[1:].view(g.shape).copy_(g)
+    wide = torch.empty(2, 2, 70, 131, device=cuda, dtype=g.dtype)[..., :128].copy_(g)
+    other = g.transpose(2, 3).contiguous().transpose(2, 3)
+    for d in (off, wide, other):
+        for a, b in zip(expected, ops.window_attention_backward(q, k, v, out, lse, d, 0.1, window=30)):
+            assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """A cache, queries and gradients whose batches lie more than 2^31 elements apart."""
+    far = 2 ** 31 + 4096
+    memory = torch.zeros(far + (1 << 20), dtype=torch.float16, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(8)
+
+    def view(heads, s, at):
+        t = memory.as_strided((2, heads, s, 128), (far, s * 128, 128, 1), at)
+        return t.copy_(torch.randn(2, heads, s, 128, generator=gen, device=cuda))
+
+    k, v, q, g = view(2, 600, 0), view(2, 600, 200000), view(4, 150, 400000), view(4, 150, 500000)
+    lengths = torch.tensor([600, 333], dtype=torch.int32, device=cuda)
+    how = dict(window=100, sinks=5, kv_lengths=lengths)
+    out, lse = ops.window_attention(q, k, v, 0.09, return_lse=True, **how)
+    expected = ref.window_attention(q, k, v, 0.09, dout=g, **how)
+    grads = ops.window_attention_backward(q, k, v, out, lse, g, 0.09, **how)
+    for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+        ref.check(t, expected[name], name)
+    one = q[:, :, :1]
+    ref.check(ops.window_attention(one, k, v, 0.09, **how), ref.window_attention(one, k, v, 0.09, **how)["out"], "decode")
+
+
+def test_many_first_tokens_and_a_short_window_over_a_long_sequence(cuda):
+    """The first tokens' later queries make more items than are kept apart."""
+    both(cuda, torch.bfloat16, 1, 1, 1, 18000, 18000, 16, 128, seed=6)
+
+
 def test_gradients_against_differences(cuda):
     """Along a random direction, by the definition's own differences in 64 bits."""
     q, k, v, g, _, _ = make(cuda, torch.float16, 1, 4, 2, 150, 150, seed=3)

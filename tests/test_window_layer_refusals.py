@@ -34,6 +34,8 @@ WRONG_ATTENTION = [
     dict(v=K.bfloat16()),
     dict(q=t(2, 4, 128, 8).transpose(2, 3)),
     dict(window=0),
+    dict(window=4.5),
+    dict(sinks=1.0),
     dict(window=-5),
     dict(sinks=-1),
     dict(sinks=129),
@@ -46,10 +48,10 @@ WRONG_ATTENTION = [
 @pytest.mark.parametrize("wrong", WRONG_ATTENTION)
 def test_attention(no_device, wrong):
     args = dict(q=Q, k=K, v=K, scale=0.1, window=4) | wrong
-    with pytest.raises(ValueError):
+    with pytest.raises((ValueError, TypeError)):
         ops.window_attention(**args)
     q = args["q"]
-    with pytest.raises(ValueError):
+    with pytest.raises((ValueError, TypeError)):
         ops.window_attention_backward(out=torch.empty_like(q), lse=t(*q.shape[:3], dtype=torch.float32),
                                       dout=torch.empty_like(q), **args)
 
@@ -107,7 +109,7 @@ def attention_status(**other):
     a = dict(dtype=rt.IXB_F16, q=1 << 20, k=1 << 20, v=1 << 20, o=1 << 20, B=1, H=4, HK=2, Sq=8, Sk=16, D=128, strides=S(8192, 1024, 128),
              scale=0.1, window=4, sinks=0) | other
     s = a["strides"]
-    return rt.load().ixb_window_attention(a["dtype"], a["q"], a["k"], a["v"], a["o"], None, None, 0, a["B"], a["H"], a["HK"], a["Sq"],
+    return rt.load().ixb_window_attention(a["dtype"], a["q"], a["k"], a["v"], a["o"], None, a["B"], a["H"], a["HK"], a["Sq"],
                                           a["Sk"], a["D"], s, s, s, s, None, None, a["scale"], a["window"], a["sinks"], None, None)
 
 
