@@ -16,6 +16,11 @@
 // side: Q and dO for dK and dV, K and V for dQ.  The others' only meet their own row of results, which is replaced.
 //
 // Every wait is bounded and raises a flag in `status`; the block leaves when its copies and products have ended.
+//
+// Bound: dK/dV the chain of a step, S -> P -> dV, next S (3050 cycles of which the tensor core works 2048) and items of equal
+// length that do not fill the last round; dQ the exponentials and what lies between two items.  2 x 4096 tokens of 32/8 heads,
+// window 1024, 4 first tokens, bf16: delta 29 us, dK/dV 252, dQ 175.  Masks inside the loop of the exponentials: 296 and 211
+// (every tile pays for the selects); dQ's results and statistics by the element-wise warps 183.
 #include <atomic>
 #include "fa_window.h"
 #include "ixb/fa_backward.cuh"

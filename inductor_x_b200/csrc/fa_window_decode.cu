@@ -11,6 +11,8 @@
 // their 8 columns, since hardly more than 8 queries share a key.  K and V come out of shared memory as whole 16-byte
 // pieces: the order of the reduced dimensions of S is free, so a lane's piece of 8 dimensions is taken for four of its pairs;
 // the rows of O are free too, so a lane pairs up its pieces of two keys element by element.
+// 64 sequences of up to 16384 keys, window 4096, 32/8 heads: 143 us, 6570 GB/s (a copy 6532); 8 sequences 25 us, 5.3 TB/s; one, window
+// 1024, 5.5 us.  With the queries as the 16 rows the same within 3 %, and twice the accumulators: an SM takes 50 GB/s either way.
 #include <atomic>
 #include "fa_window.h"
 #include "ixb/tcgen05.cuh"
