@@ -40,6 +40,11 @@ inline int check_window_views(const WindowView* views, int n) {
 // fa_window_fwd.cu
 int window_prefill(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
                    float* lse, int32_t* status, cudaStream_t stream);
+// fa_window_split.cu: over how many blocks the keys of a tile of rows are shared where that is quicker (0: not, fa_window_fwd.cu), what the
+// quicker of the two promises to take, and the call
+int window_split_size(const WindowShape& a, double* us);
+int window_split(int cluster, const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,
+                 float* lse, int32_t* status, cudaStream_t stream);
 // fa_window_decode.cu: whether it takes a call, and the call
 bool window_decodes(const WindowShape& a);
 int window_decode(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,

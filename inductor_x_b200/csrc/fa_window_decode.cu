@@ -407,12 +407,10 @@ static int clusters_of(long long items, long long tiles, int sms) {
   return cluster;
 }
 
-// Whether this kernel promises to be quicker than fa_window_fwd.cu, as measured on one B200 (35 shapes of 16 to 128 rows a key
-// head, 8 to 512 key heads, within 15 %), in us:
-//   that one   8 + 1.7 a step of 128 keys for each round of its items over the SMs
-//   this one   5 + 0.6 a tile of a warp, and not less than 1.25 for each 8 tiles an SM
-// 16 rows, 8 key heads, 1024 keys 24.2 against 6.8, 4096 keys 63 and 12.3; 64 rows, 64 key heads, 1024 keys 24.6 and 23.2, 256 key heads,
-// 2048 keys 71 and 142; 128 rows, 8 key heads, 4096 keys 62 and 23, 64 key heads, 1024 keys 24.9 and 44.5.
+// Whether this kernel promises to be quicker than the other two, as measured on one B200 (35 shapes of 16 to 128 rows a key head, 8
+// to 512 key heads, within 15 %): 5 us + 0.6 a tile of a warp, and not less than 1.25 for each 8 tiles an SM.
+// Against fa_window_fwd.cu: 16 rows, 8 key heads, 1024 keys 6.8 and 24.2, 4096 keys 12.3 and 63; 64 rows, 64 key heads, 1024 keys 23.2
+// and 24.6, 256 key heads, 2048 keys 142 and 71; 128 rows, 8 key heads, 4096 keys 23 and 62, 64 key heads, 1024 keys 44.5 and 24.9.
 bool window_decodes(const WindowShape& a) {
   const long long share = a.H / a.HK, rows = share * a.Sq;
   if (rows > 256) return false;
@@ -423,11 +421,9 @@ bool window_decodes(const WindowShape& a) {
   const long long tiles = ((long long)keys + 2 * kTile - 2) / kTile;
   const int cluster = clusters_of((long long)heads * groups, tiles, dev->sm_count);
   const double chain = 0.6 * tiles / (kWarps * cluster), load = 1.25 * heads * groups * tiles / (8 * sms);
-  int rows_of_head = 8;
-  while (rows_of_head < 128 && rows_of_head < a.Sq) rows_of_head *= 2;
-  const double pairs = ceil((double)((a.Sq + 127) / 128) * ceil((double)share * rows_of_head / 128) / 2);
-  const double steps = ceil(keys / 128) + (a.sinks > 0 ? 2 : 1);
-  return 5 + (chain > load ? chain : load) < 8 + 1.7 * steps * ceil(heads * pairs / sms);
+  double other;
+  window_split_size(a, &other);
+  return 5 + (chain > load ? chain : load) < other;
 }
 
 int window_decode(const WindowShape& a, const WindowView& q, const WindowView& k, const WindowView& v, const WindowView& o,

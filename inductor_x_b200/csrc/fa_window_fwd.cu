@@ -53,26 +53,6 @@ struct WinParams {
   int head_group;        // key heads whose items are dispatched together
 };
 
-// Of a row at position `at`: keys of the tile behind `lim` are hidden, and those in [from, low), the ones between the first
-// tokens and the window.
-struct WindowMask {
-  bool edge;
-  int lim, from, low;
-  template <int COLS> __device__ __forceinline__ void apply(uint32_t (&raw)[COLS]) const {
-    if (!edge) return;
-    // the first n keys of 32
-    auto first = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
-#pragma unroll
-    for (int c = 0; c < COLS / 32; ++c) {
-      const uint32_t seen = first(lim + 1 - c * 32) & ~(first(low - c * 32) & ~first(from - c * 32));
-      if (__all_sync(kFull, seen == 0xffffffffu)) continue;
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (!(seen >> e & 1u)) raw[c * 32 + e] = 0xff800000u;  // -inf
-    }
-  }
-};
-
 template <bool IS_BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     fa_window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -541,5 +521,8 @@ extern "C" int ixb_window_attention(int dtype, const void* q, const void* k, con
   const ixb_host::WindowShape a{dtype == IXB_BF16, B, H, HK, Sq, Sk, q_lengths, kv_lengths, scale, window < Sk ? window : Sk, sinks};
   if (ixb_host::window_decodes(a))
     return ixb_host::window_decode(a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
+  double us;
+  if (const int cluster = ixb_host::window_split_size(a, &us))
+    return ixb_host::window_split(cluster, a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
   return ixb_host::window_prefill(a, views[0], views[1], views[2], views[3], lse, status, (cudaStream_t)stream);
 }

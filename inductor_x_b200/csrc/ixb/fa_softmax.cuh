@@ -44,6 +44,26 @@ struct CausalMask {
   }
 };
 
+// Of a row at position `at`: keys of the tile behind `lim` are hidden, and those in [from, low), the ones between the first
+// tokens and the window.
+struct WindowMask {
+  bool edge;
+  int lim, from, low;
+  template <int COLS> __device__ __forceinline__ void apply(uint32_t (&raw)[COLS]) const {
+    if (!edge) return;
+    // the first n keys of 32
+    auto first = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
+#pragma unroll
+    for (int c = 0; c < COLS / 32; ++c) {
+      const uint32_t seen = first(lim + 1 - c * 32) & ~(first(low - c * 32) & ~first(from - c * 32));
+      if (__all_sync(kFull, seen == 0xffffffffu)) continue;
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (!(seen >> e & 1u)) raw[c * 32 + e] = 0xff800000u;  // -inf
+    }
+  }
+};
+
 // Scores of this thread's row (tensor memory at s_addr) to probabilities relative to the running reference
 // maximum m_used, written over them as 16-bit pairs and handed over in two parts (p_full after kSplit keys,
 // p_rest); l grows by their sum.  `mask` hides keys of the tile from this row.  `first`: the row's accumulator at

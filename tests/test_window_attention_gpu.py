@@ -286,3 +286,46 @@ def test_lengths_are_read_when_the_kernel_runs(cuda):
         graph.replay()
         torch.cuda.synchronize()
         ref.check(out, ref.window_attention(q, k, v, 0.1, window=64, sinks=2, kv_lengths=[n, n])["out"], "out")
+
+
+FEW_TILES = [
+    # B, H, HK, Sq, Sk, window, sinks, lengths of the queries, of the keys: few tiles of rows over many keys
+    (1, 4, 2, 200, 1500, 600, 4, None, None),
+    (1, 8, 2, 512, 4096, 2048, 4, None, None),
+    (2, 4, 1, 300, 2500, 5000, 0, [300, 129], [2500, 129]),
+    (1, 2, 2, 140, 9000, 8000, 128, None, None),
+    (1, 1, 1, 1024, 1024, 4096, 0, None, None),
+    (3, 3, 1, 140, 1300, 1100, 9, [140, 1, 77], [1300, 1153, 0]),       # a first token's tile, a last tile of one key
+    (4, 2, 2, 260, 1200, 700, 1, [260, 128, 129, 5], [1200, 128, 100, 1025]),
+    (1, 6, 1, 100, 2000, 1900, 128, [100], [1999]),                     # (a tile holds rows of one head, heads of it are missing)
+    (2, 5, 1, 60, 3100, 3000, 0, [60, 59], [3100, 2944]),
+    (1, 7, 1, 130, 700, 1, 1, None, None),
+    (3, 16, 8, 130, 1300, 1200, 3, None, [1300, 1153, 700]),             # as many tiles as SMs: one block a tile
+    (3, 8, 4, 200, 1500, 1300, 4, [200, 128, 0], None),                  # two
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", FEW_TILES)
+def test_few_tiles_over_many_keys(cuda, dtype, case):
+    both(cuda, dtype, *case, storage="bshd" if case[1] % 2 else "bhsd", seed=case[3])
+
+
+def test_few_tiles_on_two_streams_and_in_a_graph(cuda):
+    calls = [make(cuda, torch.bfloat16, 1, 4, 2, s, 2000, seed=s)[:3] for s in (256, 400)]
+    run = lambda i: ops.window_attention(*calls[i], 0.09, window=1500, sinks=4)
+    expected = [run(0), run(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, run(i)))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = [(i, run(i)) for i in (0, 1)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, expected[i]) for i, o in got + captured)
