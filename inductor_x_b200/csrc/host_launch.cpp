@@ -423,6 +423,7 @@ PyObject* axial_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t at_strides[3] = {pos->stride(0), all ? 0 : pos->stride(1), pos->stride(-1)};
     at::Tensor qo = at::empty_like(*q), ko;
     if (k != nullptr) ko = at::empty_like(*k);
+    if (qo.stride(3) != 1 || (k != nullptr && ko.stride(3) != 1)) Py_RETURN_NONE;  // (of an overlapping input: left to Python)
     const Strides qs(*q), qos(qo), ks(k ? *k : *q), kos(k ? ko : qo);
     const ixb_stream stream = stream_of(*q);
     const c10::OptionalDeviceGuard device(q->device());

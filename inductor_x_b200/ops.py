@@ -527,8 +527,9 @@ def _rotary_plan(sections: tuple, base: float, ladder: str, frequencies: Optiona
 
 
 def _rotary_result(t: torch.Tensor) -> torch.Tensor:
-    """In the memory order of the input; an expanded input's is a dense tensor of its own."""
-    return torch.empty_like(t) if all(t.stride()) else t.new_empty(t.shape)
+    """In the memory order of the input; an expanded or overlapping input's is a dense tensor of its own."""
+    like = torch.empty_like(t) if all(t.stride()) else t.new_empty(t.shape)
+    return like if t.dim() != 4 or like.stride(3) == 1 else t.new_empty(t.shape)
 
 
 def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inverse):

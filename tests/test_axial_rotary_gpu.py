@@ -118,3 +118,17 @@ def test_streams_graphs_and_nothing_to_do(cuda):
         assert torch.equal(a, b) and torch.equal(a, c)
     none, _ = ops.axial_rotary(q[:, :, :0], k[:, :, :0], positions[:, :, :0], [16, 24, 24])
     assert none.shape == (2, 8, 0, 128)
+
+
+@pytest.mark.parametrize("strides", [(1000, 300, 1, 1), (2000, 1, 10, 1), (1, 1, 1, 1), (32, 64, 5, 1)])
+def test_views_whose_rows_overlap(cuda, strides):
+    """(the memory order of such a view is no order for a result)"""
+    q = torch.randn(5000, device=cuda).as_strided((2, 3, 5, 64), strides)
+    k = torch.randn(2, 1, 5, 64, device=cuda)
+    positions = torch.randint(0, 500, (1, 2, 5), device=cuda)
+    for f in (ops.axial_rotary, ops.axial_rotary_backward):
+        got = f(q, k, positions, [32])
+        assert got[0].stride(3) == 1
+        for a, b in zip(got, f(q.contiguous(), k, positions, [32])):
+            assert torch.equal(a, b)
+    assert torch.equal(ops.axial_rotary(k, q[:, :1], positions, [32])[1], ops.axial_rotary(q[:, :1].contiguous(), None, positions, [32]))
