@@ -70,7 +70,8 @@ def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, 
     """One token of each sequence: the residual is added and normalised to 8 bits, projected, turned and written to the
     cache at ``lengths`` (int32 [B], which it then advances), and attends to what its window leaves of the cache.
     x, residual [B, hidden]; w: dict with norm1 and, from :func:`quantise_rows`, wqkv, and wo; positions [axes, B, 1];
-    cache_k, cache_v [B, kv_heads, capacity, D].  Returns the output projection and the new residual."""
+    cache_k, cache_v [B, kv_heads, capacity, D].  Returns the output projection and the new residual.  A sequence whose cache has
+    no room (nothing waits for the device to say so) keeps its cache and its length, and its projection is NaN."""
     from . import ops
 
     B = x.shape[0]
@@ -81,9 +82,11 @@ def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, 
     qkv = torch._scaled_mm(h8, w8.t(), scale_a=scales[:, None], scale_b=w_scales.t(), out_dtype=x.dtype)
     q, k, v = (t.view(B, 1, -1, D).transpose(1, 2) for t in qkv.split([heads * D, kv_heads * D, kv_heads * D], dim=1))
     q, k = ops.axial_rotary(q, k, positions, sections, base=base)
-    rows = torch.arange(B, device=x.device)
-    cache_k[rows, :, lengths.long()] = k[:, :, 0]
-    cache_v[rows, :, lengths.long()] = v[:, :, 0]
-    lengths += 1
+    # a sequence without room writes back what its last place holds
+    rows, room = torch.arange(B, device=x.device), (lengths >= 0) & (lengths < cache_k.shape[2])
+    place = lengths.clamp(0, cache_k.shape[2] - 1).long()
+    for cache, new in ((cache_k, k), (cache_v, v)):
+        cache[rows, :, place] = torch.where(room[:, None, None], new[:, :, 0], cache[rows, :, place])
+    lengths += room
     a = ops.window_attention(q, cache_k, cache_v, 1.0 / math.sqrt(D), window=window, sinks=sinks, kv_lengths=lengths)
-    return F.linear(a.view(B, heads * D), w["wo"]), residual
+    return F.linear(a.view(B, heads * D), w["wo"]).masked_fill(~room[:, None], math.nan), residual

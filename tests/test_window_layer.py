@@ -187,3 +187,27 @@ def test_serving_steps_over_a_cache(cuda):
     value, bound = ref.window_attention(q, cache_k, cache_v, 1 / math.sqrt(D), kv_lengths=lengths, **how)["out"]
     ref.check(together, (value, bound), "at once")
     ref.check(steps, (value, bound), "one by one")
+
+
+@pytest.mark.gpu
+def test_a_serving_step_without_room(cuda):
+    """A full cache, and a length that is none, stay as they are; the others are served as they are without them."""
+    B, hidden, H, K, D, capacity = 4, 256, 4, 2, 128, 20
+    w = weights(cuda, torch.bfloat16, hidden, H, K)
+    w8 = {"norm1": w["norm1"], "wqkv": llama_layer.quantise_rows(torch.cat([w["wq"], w["wk"], w["wv"]])), "wo": w["wo"]}
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    new = lambda *shape: torch.randn(*shape, generator=gen, device=cuda).bfloat16()  # noqa: E731
+    caches, x, residual = [new(B, K, capacity, D) for _ in range(2)], new(B, hidden), new(B, hidden)
+    how = dict(heads=H, kv_heads=K, sections=(64,), window=8, sinks=2)
+
+    def step(lengths):
+        lengths, here = torch.tensor(lengths, dtype=torch.int32, device=cuda), [c.clone() for c in caches]
+        y, _ = llama_layer.window_attention_step(x, residual, w8, lengths.clamp(min=0).long()[None, :, None], *here, lengths, **how)
+        return y, here, lengths.tolist()
+
+    y, here, lengths = step([20, 19, -1, 5])
+    expected, there, _ = step([3, 19, 4, 5])
+    assert lengths == [20, 20, -1, 6]
+    assert bool(y[[0, 2]].isnan().all()) and torch.equal(y[[1, 3]], expected[[1, 3]])
+    for c, a, b in zip(caches, here, there):
+        assert torch.equal(a[[0, 2]], c[[0, 2]]) and torch.equal(a[[1, 3]], b[[1, 3]])
