@@ -362,7 +362,9 @@ def rmsnorm_quantised(x, w, eps: float = 1e-6, *, residual=None, return_residual
     if not x.is_contiguous() or x.dim() < 1:
         raise ValueError("x must be contiguous")
     cols = x.shape[-1]
-    rows = x.numel() // cols if cols else 0
+    if cols == 0:
+        raise ValueError("a row must have a value")
+    rows = x.numel() // cols
     if w.shape != (cols,) or w.dtype != x.dtype:
         raise ValueError("w must be a vector of length cols in x's dtype")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype

@@ -147,3 +147,9 @@ def test_other_entries():
     assert norm(x=None) == rt.IXB_ERR_ARG and norm(h=1) == rt.IXB_ERR_ARG and norm(group=64) == rt.IXB_ERR_ARG
     assert norm(rows=-1) == rt.IXB_ERR_ARG and norm(cols=0) == rt.IXB_ERR_ARG and norm(rows=0, x=None) == rt.IXB_OK
     assert norm(cols=1 << 21) == rt.IXB_ERR_SHAPE and norm(dtype=rt.IXB_I64) == rt.IXB_ERR_DTYPE
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_norm_of_rows_without_values(no_device, group):
+    with pytest.raises(ValueError):
+        ops.rmsnorm_quantised(t(4, 0), t(0), group=group)
