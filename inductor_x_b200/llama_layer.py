@@ -65,11 +65,23 @@ def quantise_rows(weight: torch.Tensor):
     return (weight.float() / scales).to(torch.float8_e4m3fn), scales
 
 
+def _scaled_product(h8, scales, weight, dtype):
+    """``(h8 * scales) @ (w8 * w_scales)^T`` in ``dtype``: a plain library product of 8-bit values whose results take a row's and
+    a column's scale.  With those scales the library rounds to bf16 only (asked for fp16 it returns values that are off by as much
+    as the largest); for fp16 its unscaled 32-bit sums are scaled here and rounded once."""
+    w8, w_scales = weight
+    if dtype == torch.bfloat16:
+        return torch._scaled_mm(h8, w8.t(), scale_a=scales[:, None], scale_b=w_scales.t(), out_dtype=dtype)
+    one = scales.new_ones(())
+    sums = torch._scaled_mm(h8, w8.t(), scale_a=one, scale_b=one, out_dtype=torch.float32)
+    return (sums * scales[:, None] * w_scales.t()).to(dtype)
+
+
 def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, *, heads: int, kv_heads: int, sections,
                           window: int, sinks: int = 0, base: float = 10000.0, eps: float = 1e-6):
     """One token of each sequence: the residual is added and normalised to 8 bits, projected, turned and written to the
     cache at ``lengths`` (int32 [B], which it then advances), and attends to what its window leaves of the cache.
-    x, residual [B, hidden]; w: dict with norm1 and, from :func:`quantise_rows`, wqkv, and wo; positions [axes, B, 1];
+    x, residual [B, hidden], bf16 or fp16; w: dict with norm1 and, from :func:`quantise_rows`, wqkv, and wo; positions [axes, B, 1];
     cache_k, cache_v [B, kv_heads, capacity, D].  Returns the output projection and the new residual.  A sequence whose cache has
     no room (nothing waits for the device to say so) keeps its cache and its length, and its projection is NaN."""
     from . import ops
@@ -77,9 +89,7 @@ def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, 
     B = x.shape[0]
     D = cache_k.shape[3]
     h8, scales, residual = ops.rmsnorm_quantised(x, w["norm1"], eps, residual=residual, return_residual=True)
-    w8, w_scales = w["wqkv"]
-    # (a row and a column scale: a plain library product)
-    qkv = torch._scaled_mm(h8, w8.t(), scale_a=scales[:, None], scale_b=w_scales.t(), out_dtype=x.dtype)
+    qkv = _scaled_product(h8, scales, w["wqkv"], x.dtype)
     q, k, v = (t.view(B, 1, -1, D).transpose(1, 2) for t in qkv.split([heads * D, kv_heads * D, kv_heads * D], dim=1))
     q, k = ops.axial_rotary(q, k, positions, sections, base=base)
     # a sequence without room writes back what its last place holds
