@@ -82,12 +82,15 @@ def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, 
     """One token of each sequence: the residual is added and normalised to 8 bits, projected, turned and written to the
     cache at ``lengths`` (int32 [B], which it then advances), and attends to what its window leaves of the cache.
     x, residual [B, hidden], bf16 or fp16; w: dict with norm1 and, from :func:`quantise_rows`, wqkv, and wo; positions [axes, B, 1];
-    cache_k, cache_v [B, kv_heads, capacity, D].  Returns the output projection and the new residual.  A sequence whose cache has
+    cache_k, cache_v [B, kv_heads, capacity, D], as :func:`ops.window_attention` takes them.  Returns the output projection and the new residual.  A sequence whose cache has
     no room (nothing waits for the device to say so) keeps its cache and its length, and its projection is NaN."""
     from . import ops
 
-    B = x.shape[0]
-    D = cache_k.shape[3]
+    # a call that is refused leaves the cache and the lengths as they are
+    B, D = x.shape[0], cache_k.shape[-1]
+    ops._window_arguments(x.new_empty(B, heads, 0, D), cache_k, cache_v, window, sinks, None, lengths)
+    if cache_k.shape[1] != kv_heads or cache_k.shape[2] == 0 or not (ops._operand_fits(cache_k) and ops._operand_fits(cache_v)):
+        raise ValueError("the caches must be [B, kv_heads, capacity, D] with strides of whole 16 bytes")
     h8, scales, residual = ops.rmsnorm_quantised(x, w["norm1"], eps, residual=residual, return_residual=True)
     qkv = _scaled_product(h8, scales, w["wqkv"], x.dtype)
     q, k, v = (t.view(B, 1, -1, D).transpose(1, 2) for t in qkv.split([heads * D, kv_heads * D, kv_heads * D], dim=1))

@@ -398,6 +398,12 @@ def _operand_strides(t: torch.Tensor):
     return _I64x3(b if B > 1 else H * S * D, h, s)
 
 
+def _operand_fits(t: torch.Tensor) -> bool:
+    """Whether the attention kernels take a tensor as it lies: ``D`` contiguous, other strides positive multiples of 8 elements, rows
+    on 16-byte boundaries."""
+    return t.numel() == 0 or (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st > 0 and st % 8 == 0 for st in _operand_strides(t)))
+
+
 def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
     _need_cuda(q, k, v, q_lengths, kv_lengths, *more)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -483,8 +489,7 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError("lse must be float32 [B, H, Sq]")
     _one_device(q, out, lse, dout)
     lse = lse.contiguous()
-    if dout.numel() and (dout.stride(3) != 1 or any(st <= 0 or st % 8 for st in _operand_strides(dout))
-                         or dout.data_ptr() % 16):
+    if not _operand_fits(dout):
         dout = dout.clone(memory_format=torch.contiguous_format)
     if out.numel() and out.stride(3) != 1:
         raise ValueError("the head dimension must be contiguous")

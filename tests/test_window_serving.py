@@ -55,3 +55,39 @@ def test_step(cuda, monkeypatch, dtype, B):
     z, bound = a @ b.t(), (H * D + 1) * 2.0 ** -24 * (a.abs() @ b.abs().t())
     ref.check(y, (z, bound * (1 + half) + half * z.abs() + ref._floor(dtype)), "y")
     assert bool(torch.isfinite(y).all())
+
+
+def _refused(**other):
+    """A step on host memory that has to be refused before anything is computed (there are no weights)."""
+    cache = lambda: torch.zeros(3, K, 20, D, dtype=torch.float16)  # noqa: E731
+    a = dict(x=torch.zeros(3, HIDDEN, dtype=torch.float16), cache_k=cache(), cache_v=cache(), lengths=torch.full((3,), 4, dtype=torch.int32)) | HOW | other
+    with pytest.raises(ValueError):
+        llama_layer.window_attention_step(a.pop("x"), None, {}, None, a.pop("cache_k"), a.pop("cache_v"), a.pop("lengths"), **a)
+
+
+@pytest.mark.parametrize("other", [
+    dict(lengths=torch.full((3,), 4)), dict(lengths=torch.full((2,), 4, dtype=torch.int32)), dict(window=0), dict(sinks=129), dict(kv_heads=1),
+    dict(heads=5), dict(cache_k=torch.zeros(3, K, 20, D)), dict(cache_v=torch.zeros(3, K, 21, D, dtype=torch.float16)),
+    dict(cache_k=torch.zeros(2, K, 20, D, dtype=torch.float16), cache_v=torch.zeros(2, K, 20, D, dtype=torch.float16)),
+    dict(x=torch.zeros(3, HIDDEN)), dict(cache_k=torch.zeros(3, K, 20, D + 4, dtype=torch.float16)[..., :D]),
+    dict(cache_k=torch.zeros(3, K, 0, D, dtype=torch.float16), cache_v=torch.zeros(3, K, 0, D, dtype=torch.float16)),
+    dict(cache_v=torch.zeros(1, K, 20, D, dtype=torch.float16).expand(3, K, 20, D))])
+def test_refusals_come_before_anything_is_computed(monkeypatch, other):
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "rmsnorm_quantised", lambda *a, **k: pytest.fail("a call that had to be refused was made"))
+    _refused(**other)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wrong", [dict(window=0), dict(sinks=129), dict(kind=torch.int64), dict(pitch=4)])
+def test_what_is_refused_changes_nothing(cuda, wrong):
+    gen = torch.Generator(device=cuda).manual_seed(7)
+    w = weights(cuda, torch.bfloat16, gen)
+    caches = [torch.randn(2, K, 30, D + wrong.get("pitch", 0), generator=gen, device=cuda).bfloat16()[..., :D] for _ in range(2)]
+    x = torch.randn(2, HIDDEN, generator=gen, device=cuda).bfloat16()
+    lengths = torch.tensor([3, 29], device=cuda, dtype=wrong.get("kind", torch.int32))
+    before = [t.clone() for t in (*caches, lengths)]
+    with pytest.raises(ValueError):
+        llama_layer.window_attention_step(x, x, w, torch.zeros(3, 2, 1, dtype=torch.int64, device=cuda), *caches, lengths,
+                                          **(HOW | {n: v for n, v in wrong.items() if n in HOW}))
+    assert all(torch.equal(a, b) for a, b in zip(before, (*caches, lengths)))
