@@ -320,8 +320,8 @@ int ixb_window_attention_bwd(int dtype, const void* q, const void* k, const void
  * order, at most 128 together and 2 * pairs <= D; frequencies[pairs] (host memory): radians a position.  Pair i of
  * a head is turned by positions[axis(i), b, s] * frequencies[i], the angle formed in 64 bits; pair i is
  * (i, pairs + i), or (2i, 2i + 1) with neighbours != 0; what lies behind the pairs is copied.  inverse != 0 turns the
- * other way: the gradient.  positions I64 or I32 with the strides of its three axes in elements; B * S at most 2^30.  The reference has
- * rotary embeddings as pointwise graphs only (inductor_x/lowering.py:45-88). */
+ * other way: the gradient.  positions I64 or I32 with the strides of its three axes in elements; B * S
+ * and (heads + k_heads) * D at most 2^30 each.  The reference has rotary embeddings as pointwise graphs only (inductor_x/lowering.py:45-88). */
 int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int64_t* q_strides,
                      const int64_t* q_out_strides, int32_t heads, const void* k, void* k_out,
                      const int64_t* k_strides, const int64_t* k_out_strides, int32_t k_heads,

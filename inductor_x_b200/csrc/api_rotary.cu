@@ -224,7 +224,8 @@ extern "C" int ixb_axial_rotary(int dtype, const void* q, void* q_out, const int
   }
   if (2 * p.pairs > D) return IXB_ERR_SHAPE;
   if (B == 0 || S == 0 || D == 0 || heads + (long long)k_heads == 0) return IXB_OK;
-  if ((long long)B * S > (1 << 30)) return IXB_ERR_SHAPE;
+  // (the kernels count a token's values, and the tokens, in 32 bits)
+  if ((long long)B * S > (1 << 30) || (heads + (long long)k_heads) * D > (1 << 30)) return IXB_ERR_SHAPE;
   if ((heads && (!q || !q_out || !q_strides || !q_out_strides)) || (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) ||
       !positions || !position_strides)
     return IXB_ERR_ARG;

@@ -415,7 +415,7 @@ PyObject* axial_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (k != nullptr && (!dense(*k) || !alike(*q, *k) || k->size(0) != q->size(0) || k->size(2) != q->size(2) || k->size(3) != q->size(3)))
       Py_RETURN_NONE;
     const int64_t B = q->size(0), S = q->size(2);
-    if (B * S > INT32_MAX || q->size(1) > INT32_MAX || (k != nullptr && k->size(1) > INT32_MAX)) Py_RETURN_NONE;
+    if (B * S > INT32_MAX || q->size(1) > INT32_MAX || q->size(3) > INT32_MAX || (k != nullptr && k->size(1) > INT32_MAX)) Py_RETURN_NONE;
     const bool all = pos->dim() == 2;
     if ((!all && pos->dim() != 3) || pos->size(0) != axes || (!all && pos->size(1) != B) || pos->size(-1) != S ||
         (pos->scalar_type() != at::kLong && pos->scalar_type() != at::kInt))

@@ -389,6 +389,12 @@ def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
             raise ValueError("all tensors must be on one device")
 
 
+def _fits_32_bits(*ts: Optional[torch.Tensor]) -> None:
+    """The entries take an axis as a 32-bit number (views of few bytes may have longer ones)."""
+    if any(t is not None and any(n > 2 ** 31 - 1 for n in t.shape) for t in ts):
+        raise ValueError("an axis may not have more than 2^31 - 1 entries")
+
+
 def _operand_strides(t: torch.Tensor):
     """Strides of the (batch, head, sequence) axes; an axis of one entry, whose stride says nothing, counts as dense."""
     B, H, S, D = t.shape
@@ -412,6 +418,7 @@ def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
         raise ValueError("the query heads must be a multiple of the key heads")
     if q.shape[3] != 128:
         raise ValueError("the head dimension must be 128")
+    _fits_32_bits(q, k)
     if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v, *more)):
         raise ValueError("q, k, v (and out, dout) must share dtype float16 or bfloat16")
     window, sinks = operator.index(window), operator.index(sinks)
@@ -553,6 +560,7 @@ def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inver
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
         raise ValueError("expected q[B,H,S,D], k[B,HK,S,D]")
     B, H, S, D = q.shape
+    _fits_32_bits(q, k)
     if 2 * pairs > D:
         raise ValueError("the sections turn more than the head dimension has")
     if positions.dtype not in (torch.int64, torch.int32) or positions.shape not in ((axes, B, S), (axes, S)):
