@@ -523,6 +523,7 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 PAIRINGS, LADDERS = ("halves", "neighbours"), ("shared", "own")
 
 
+# (kept by value: whole numbers and floats only, so that no entry holds a caller's tensor)
 @functools.lru_cache(maxsize=256)
 def _rotary_plan(sections: tuple, base: float, ladder: str, frequencies: Optional[tuple]):
     """(pairs, axes, ctypes sections, ctypes frequencies in radians a position, their addresses)."""
@@ -550,7 +551,7 @@ def _rotary(q, k, positions, sections, base, pairing, ladder, frequencies, inver
     if pairing not in PAIRINGS or ladder not in LADDERS:
         raise ValueError(f"pairing must be one of {PAIRINGS}, ladder one of {LADDERS}")
     pairs, axes, c_sections, c_frequencies, *addresses = _rotary_plan(
-        tuple(sections), float(base), ladder, tuple(frequencies) if frequencies is not None else None)
+        tuple(map(operator.index, sections)), float(base), ladder, tuple(map(float, frequencies)) if frequencies is not None else None)
     done = _native("ixb_axial_rotary", _ixb_host.axial_rotary(q, k, positions, pairs, axes, *addresses, pairing == "neighbours", inverse))
     if done is not None:
         return done
