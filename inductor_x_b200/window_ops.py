@@ -22,7 +22,7 @@ b200_def.define("b200_window_attention_backward(Tensor query, Tensor key, Tensor
                 "float scale, int window, int sinks=0, Tensor? q_lengths=None, Tensor? kv_lengths=None) "
                 "-> (Tensor, Tensor, Tensor)")
 b200_def.define("b200_axial_rotary(Tensor query, Tensor key, Tensor positions, int[] sections, float base=10000., "
-                "str pairing='halves', str ladder='shared', bool inverse=False) -> (Tensor, Tensor)")
+                "str pairing='halves', str ladder='shared', bool inverse=False, float[]? frequencies=None) -> (Tensor, Tensor)")
 b200_def.define("b200_rmsnorm_quantised(Tensor x, Tensor weight, float eps, Tensor? residual=None, int group=0) "
                 "-> (Tensor, Tensor, Tensor)")
 
@@ -66,17 +66,19 @@ def _window_gradient(ctx, dout, _):
 
 
 # ---- rotary positions --------------------------------------------------------------------------------
-def _axial_rotary(query, key, positions, sections, base=10000.0, pairing="halves", ladder="shared", inverse=False):
+def _axial_rotary(query, key, positions, sections, base=10000.0, pairing="halves", ladder="shared", inverse=False,
+                  frequencies=None):
     turn = ops.axial_rotary_backward if inverse else ops.axial_rotary
-    return turn(query, key, positions, sections, base=base, pairing=pairing, ladder=ladder)
+    return turn(query, key, positions, sections, base=base, pairing=pairing, ladder=ladder, frequencies=frequencies)
 
 
-def _axial_rotary_meta(query, key, positions, sections, base=10000.0, pairing="halves", ladder="shared", inverse=False):
+def _axial_rotary_meta(query, key, positions, sections, base=10000.0, pairing="halves", ladder="shared", inverse=False,
+                       frequencies=None):
     return ops._rotary_result(query), ops._rotary_result(key)
 
 
 def _rotary_setup(ctx, inputs, output):
-    _, _, positions, ctx.sections, ctx.base, ctx.pairing, ctx.ladder, ctx.inverse = inputs
+    _, _, positions, ctx.sections, ctx.base, ctx.pairing, ctx.ladder, ctx.inverse, ctx.frequencies = inputs
     ctx.save_for_backward(positions)
 
 
@@ -84,8 +86,8 @@ def _rotary_gradient(ctx, dq, dk):
     (positions,) = ctx.saved_tensors
     dense = lambda t: t if t.stride(3) == 1 or t.numel() == 0 else t.contiguous()  # noqa: E731  (the gradient of a sum has no strides)
     dq, dk = torch.ops.b200_graph.b200_axial_rotary(dense(dq), dense(dk), positions, ctx.sections, ctx.base, ctx.pairing,
-                                                    ctx.ladder, not ctx.inverse)
-    return dq, dk, None, None, None, None, None, None
+                                                    ctx.ladder, not ctx.inverse, ctx.frequencies)
+    return dq, dk, None, None, None, None, None, None, None
 
 
 # ---- norm with an 8-bit output -----------------------------------------------------------------------
