@@ -441,9 +441,10 @@ def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, window: int, sinks: int = 0,
                      q_lengths: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
                      return_lse: bool = False, check: bool = False):
-    """Causal attention of ``q[B, H, Sq, D]`` over ``k``, ``v`` ``[B, HK, Sk, D]`` (``H`` a multiple of ``HK``, any
-    batch/head/sequence strides, ``D`` contiguous, ``D == 128``, fp16 or bf16) in which a query sees the last
-    ``window`` keys up to its own position and the first ``sinks`` (at most 128) of the sequence.
+    """Causal attention of ``q[B, H, Sq, D]`` over ``k``, ``v`` ``[B, HK, Sk, D]`` (``H`` a multiple of ``HK``, ``D`` contiguous,
+    ``D == 128``, fp16 or bf16, batch/head/sequence strides that are positive multiples of 8 elements, the first element on a
+    16-byte boundary; other operands are refused, and made dense by ``b200_graph::b200_window_attention``) in which a query
+    sees the last ``window`` keys up to its own position and the first ``sinks`` (at most 128) of the sequence.
 
     ``q_lengths`` and ``kv_lengths`` (int32 ``[B]`` on the device; all of ``Sq`` and ``Sk`` without) are the lengths of
     a padded batch or of what a cache holds: query ``i`` stands at position ``kv_lengths[b] - q_lengths[b] + i``, the
@@ -479,7 +480,7 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               q_lengths: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
                               check: bool = False):
     """Gradients ``(dq, dk, dv)`` of :func:`window_attention` from its inputs, its output ``out``, its log-sum-exp
-    ``lse`` (``return_lse=True``) and the incoming gradient ``dout``; ``dk`` and ``dv`` are sums over the query heads
+    ``lse`` (``return_lse=True``) and the incoming gradient ``dout`` (any strides; the others' as there); ``dk`` and ``dv`` are sums over the query heads
     that share a key head, and zero where no query sees the key.  Deterministic, no atomics."""
     if not check:
         done = _native("ixb_window_attention_bwd", _ixb_host.window_attention_backward(

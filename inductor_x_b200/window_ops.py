@@ -28,8 +28,13 @@ b200_def.define("b200_rmsnorm_quantised(Tensor x, Tensor weight, float eps, Tens
 
 
 # ---- windowed attention ----------------------------------------------------------------------------
+def _fit(t):
+    """As it is where the kernels take it so, else dense (an expanded or oddly sliced operand; the functions refuse those)."""
+    return t if t.dim() != 4 or ops._operand_fits(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def _window_attention(query, key, value, scale, window, sinks=0, q_lengths=None, kv_lengths=None):
-    return ops.window_attention(query, key, value, scale, window=window, sinks=sinks, q_lengths=q_lengths,
+    return ops.window_attention(_fit(query), _fit(key), _fit(value), scale, window=window, sinks=sinks, q_lengths=q_lengths,
                                 kv_lengths=kv_lengths, return_lse=True)
 
 
@@ -39,7 +44,7 @@ def _window_attention_meta(query, key, value, scale, window, sinks=0, q_lengths=
 
 
 def _window_attention_backward(query, key, value, out, lse, dout, scale, window, sinks=0, q_lengths=None, kv_lengths=None):
-    return ops.window_attention_backward(query, key, value, out, lse, dout, scale, window=window, sinks=sinks,
+    return ops.window_attention_backward(_fit(query), _fit(key), _fit(value), _fit(out), lse, dout, scale, window=window, sinks=sinks,
                                          q_lengths=q_lengths, kv_lengths=kv_lengths)
 
 

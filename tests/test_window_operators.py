@@ -33,3 +33,44 @@ def test_frequencies(cuda, compiled, pairing):
     for x, y, dy, dx in zip((q, k), turned, g, grads):
         ref.check(y.detach(), ref.axial_rotary(x.detach(), positions, [12, 8], **how), "turned")
         ref.check(dx, ref.axial_rotary(dy, positions, [12, 8], inverse=True, **how), "gradient")
+
+
+LAYOUTS = {
+    "expanded heads": lambda t: t[:, :1].expand_as(t),
+    "expanded batch": lambda t: t[:1].expand_as(t),
+    "a slice at an odd offset": lambda t: torch.cat([t[..., :4], t], -1)[..., 4:],
+    "an odd pitch": lambda t: torch.cat([t, t[..., :3]], -1)[..., :128],
+    "off a boundary": lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape),
+    "the head dimension apart": lambda t: t.transpose(2, 3).contiguous().transpose(2, 3),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compiled", [False, True])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_attention_of_operands_in_any_layout(cuda, layout, compiled):
+    """As of dense copies, bit for bit, and so are the gradients; those of an expanded operand are summed."""
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    base = [torch.randn(2, h, s, 128, generator=gen, device=cuda).bfloat16() for h, s in ((4, 70), (2, 90), (2, 90))]
+    lengths = torch.tensor([90, 33], dtype=torch.int32, device=cuda)
+    g = torch.randn(2, 4, 70, 128, generator=gen, device=cuda).bfloat16()
+
+    def run(change, compiled):
+        leaves = [t.clone().requires_grad_() for t in base]
+        f = lambda q, k, v: G.b200_window_attention(q, k, v, 0.1, 30, 3, None, lengths)  # noqa: E731
+        torch._dynamo.reset()
+        f = torch.compile(f, fullgraph=True) if compiled else f
+        operands = [change(t) for t in leaves]
+        out, lse = f(*operands)
+        return operands, out, lse, torch.autograd.grad(out, operands, g)
+
+    operands, out, lse, grads = run(LAYOUTS[layout], compiled)
+    assert not any(ops._operand_fits(t) for t in operands)
+    dense = [t.detach().clone(memory_format=torch.contiguous_format) for t in operands]
+    how = dict(window=30, sinks=3, kv_lengths=lengths)
+    expected, e_lse = ops.window_attention(*dense, 0.1, return_lse=True, **how)
+    assert torch.equal(out, expected) and torch.equal(lse, e_lse)
+    for a, b in zip(grads, ops.window_attention_backward(*dense, expected, e_lse, g, 0.1, **how)):
+        assert torch.equal(a, b)
+    direct = torch.ops.b200_graph.b200_window_attention_backward(*operands, LAYOUTS[layout](out), lse, g, 0.1, 30, 3, None, lengths)
+    assert [t.shape for t in direct] == [t.shape for t in operands]
