@@ -145,9 +145,10 @@ int ixb_rmsnorm(int dtype, const void* x, const void* res, const void* w, void* 
 /* RMSNorm with an 8-bit output: h = x (+ res), rounded to the storage type;
  * y = h * rsqrt(mean(h*h) + eps) * w in fp32; scales = max|y| / 448 over the row (group 0: scales[rows]) or
  * over each 128 of its values (group 128: scales[rows, ceil(cols / 128)], the last over what is left);
- * q[rows, cols] = e4m3(y / scale), to the nearest.  Where scale is 0 so is q; a NaN or an infinity of y
- * makes its scale and what it covers NaN.  res and h_out may be null; rows below 2^31, cols at most 2^20.  No counterpart in the reference: its norms
- * leave 16 bits (inductor_x/lowering.py:217-233). */
+ * q[rows, cols] = e4m3(y / scale), to the nearest.  Where scale is 0 so is q.  A NaN of y makes its scale and all that
+ * the scale covers NaN; an infinity of y makes its scale infinite, itself NaN and the finite values beside it 0.  (An infinity of
+ * h makes the row's root 0: its own y is NaN, the row's others are 0.)  res and h_out may be null; rows below 2^31, cols at most 2^20.
+ * No counterpart in the reference: its norms leave 16 bits (inductor_x/lowering.py:217-233). */
 int ixb_rmsnorm_quantised(int dtype, const void* x, const void* res, const void* w, void* q,
                           float* scales, void* h_out, int64_t rows, int64_t cols, int32_t group,
                           float eps, ixb_stream stream);
@@ -286,7 +287,9 @@ int ixb_fa_bwd_scratch(int dtype, const void* q, const void* k, const void* v, c
  * strides and alignment as ixb_fa_fwd.  q_lengths and kv_lengths: int32[B] on the device or null (Sq and Sk;
  * values outside [0, Sq] and [0, Sk] count as the nearest of those).  Query i of sequence b stands at position
  * p = kv_lengths[b] - q_lengths[b] + i and sees key j when j <= p and (j > p - window or j < sinks) and
- * j < kv_lengths[b]; a query that sees nothing, and any at or behind q_lengths[b], gets o = 0 and lse = -inf.
+ * j < kv_lengths[b]; a query that sees nothing, and any at or behind q_lengths[b], gets o = 0 and lse = -inf.  What lies
+ * behind the lengths may be anything; values of v before them have to be finite, since a NaN or an infinity may reach queries that do
+ * not see its key (a weight of 0 times it).
  * lse[B,H,Sq] may be null.  window >= 1, 0 <= sinks <= 128, Sk >= 1, scale > 0 and finite.  `status` as in
  * ixb_fa_fwd.  The reference passes such bounds to the vendor kernel as pre_tockens / next_tockens
  * (inductor_x/npu_fusion_attention_graph.py:13-18). */
@@ -298,7 +301,7 @@ int ixb_window_attention(int dtype, const void* q, const void* k, const void* v,
                          int32_t* status, ixb_stream stream);
 
 /* Gradients of ixb_window_attention from its output `o` and log-sum-exp `lse`; dk and dv are summed over
- * the query heads that share a key head.  Every element of dq, dk and dv is written: zeros where nothing
+ * the query heads that share a key head.  Before the lengths q, k, v and dout have to be finite, as v there.  Every element of dq, dk and dv is written: zeros where nothing
  * was seen (B, H > 0; Sq, Sk >= 1).  No atomics: the same bits every time.  `scratch` of ixb_window_attention_bwd_scratch_bytes
  * bytes, 16-byte aligned, contents lost. */
 size_t ixb_window_attention_bwd_scratch_bytes(int32_t B, int32_t H, int32_t HK, int32_t Sq,

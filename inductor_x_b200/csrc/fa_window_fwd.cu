@@ -29,7 +29,7 @@ namespace {
 using namespace ixb;
 using namespace ixb::fa;
 
-constexpr int kFront = 32;  // keys of a short last step
+constexpr int kFront = 32;  // keys of a short step
 constexpr int kFrontBytes = kFront * HD * 2;
 constexpr int kStages = 2;  // (the issuer picks stage descriptors with two-way selects)
 // Registers: as in fa_fwd.cu

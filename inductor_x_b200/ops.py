@@ -350,7 +350,9 @@ def rmsnorm_quantised(x, w, eps: float = 1e-6, *, residual=None, return_residual
     Returns ``(q, scales)`` or ``(q, scales, h)``: ``h = x + residual`` rounded to the storage dtype, ``q``
     (``torch.float8_e4m3fn``, the shape of ``x``) times ``scales`` (float32) the norm of ``h``.  ``group=0``: a scale
     for each row, ``scales`` of shape ``x.shape[:-1]``; ``group=128``: one for each 128 values, ``[..., ceil(cols /
-    128)]``.  A scale is the largest magnitude / 448; the norm is rounded once, to 8 bits."""
+    128)]`` and contiguous (a product that wants the rows' axis innermost takes ``scales.t().contiguous().t()``).  A scale is the
+    largest magnitude / 448; the norm is rounded once, to 8 bits.  A NaN of the norm makes its scale and all that the scale
+    covers NaN, an infinity makes its scale infinite, itself NaN and the finite values beside it 0."""
     done = _native("ixb_rmsnorm_quantised", _ixb_host.rms_norm_quantised(x, w, eps, residual, return_residual, group))
     if done is not None:
         return done
@@ -410,8 +412,8 @@ def _operand_fits(t: torch.Tensor) -> bool:
     return t.numel() == 0 or (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st > 0 and st % 8 == 0 for st in _operand_strides(t)))
 
 
-def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
-    _need_cuda(q, k, v, q_lengths, kv_lengths, *more)
+def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths):
+    _need_cuda(q, k, v, q_lengths, kv_lengths)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError("expected q[B,H,Sq,D], k[B,HK,Sk,D], v[B,HK,Sk,D]")
     if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
@@ -419,8 +421,8 @@ def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
     if q.shape[3] != 128:
         raise ValueError("the head dimension must be 128")
     _fits_32_bits(q, k)
-    if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v, *more)):
-        raise ValueError("q, k, v (and out, dout) must share dtype float16 or bfloat16")
+    if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v)):
+        raise ValueError("q, k, v must share dtype float16 or bfloat16")
     window, sinks = operator.index(window), operator.index(sinks)
     if not 1 <= window:
         raise ValueError("window must be at least 1")
@@ -429,10 +431,10 @@ def _window_arguments(q, k, v, window, sinks, q_lengths, kv_lengths, more=()):
     for n in (q_lengths, kv_lengths):
         if n is not None and (n.dtype != torch.int32 or n.shape != q.shape[:1]):
             raise ValueError("lengths must be int32 [B]")
-    for t in (q, k, v, *more):
+    for t in (q, k, v):
         if t.numel() and t.stride(3) != 1:
             raise ValueError("the head dimension must be contiguous")
-    _one_device(q, k, v, q_lengths, kv_lengths, *more)
+    _one_device(q, k, v, q_lengths, kv_lengths)
     most = 2 ** 31 - 1
     return (min(window, most), sinks, q_lengths.contiguous() if q_lengths is not None else None,
             kv_lengths.contiguous() if kv_lengths is not None else None)
@@ -449,7 +451,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     ``q_lengths`` and ``kv_lengths`` (int32 ``[B]`` on the device; all of ``Sq`` and ``Sk`` without) are the lengths of
     a padded batch or of what a cache holds: query ``i`` stands at position ``kv_lengths[b] - q_lengths[b] + i``, the
     last query at the last key.  A query that sees nothing, and any behind ``q_lengths[b]``, gets zeros and a
-    log-sum-exp of ``-inf``.  One to a few queries over a long cache are a decoding step: only the keys they see
+    log-sum-exp of ``-inf``.  What lies behind the lengths may be anything; values of ``v`` before them have to be finite (a NaN
+    or an infinity may reach queries that do not see its key, as a weight of 0 times it).  One to a few queries over a long cache are a decoding step: only the keys they see
     are read.
 
     Returns ``out`` (contiguous ``[B, H, Sq, D]``) or ``(out, lse)``; ``check=True`` as in :func:`fused_attention`."""

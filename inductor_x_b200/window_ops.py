@@ -1,7 +1,8 @@
 """The operators of a decoder layer with a sliding window as PyTorch operators, for eager models, ``torch.compile`` and
 autograd:
 
-* ``b200_graph::b200_window_attention`` - :func:`ops.window_attention`, output and log-sum-exp, with its gradient;
+* ``b200_graph::b200_window_attention`` - :func:`ops.window_attention`, output and log-sum-exp, with its gradient. The log-sum-exp
+  itself is not differentiated through: it does not require a gradient, and a loss that adds a term of it gets none for that term;
 * ``b200_graph::b200_axial_rotary`` - :func:`ops.axial_rotary`, with its gradient;
 * ``b200_graph::b200_rmsnorm_quantised`` - :func:`ops.rmsnorm_quantised` (a serving operator: no gradient).
 
@@ -116,7 +117,6 @@ for _name, _cuda, _meta in (("b200_window_attention", _window_attention, _window
     b200_cuda.impl(_name, _cuda)
     b200_meta.impl(_name, _meta)
 
-# (the log-sum-exp is not differentiated through)
 torch.library.register_autograd("b200_graph::b200_window_attention", _window_gradient, setup_context=_window_setup,
                                 lib=b200_def)
 torch.library.register_autograd("b200_graph::b200_axial_rotary", _rotary_gradient, setup_context=_rotary_setup, lib=b200_def)
