@@ -25,6 +25,7 @@ import torch
 from torch._inductor import ir, lowering
 from torch._inductor.lowering import (_make_reduction_inner, _validate_reduction_axis, fallbacks,
                                       lowerings, make_fallback)
+from torch.utils._pytree import tree_leaves
 
 aten = torch.ops.aten
 prims = torch.ops.prims
@@ -146,10 +147,35 @@ def _install_scan_lowerings():
         lowerings[op] = extern
 
 
+#: no template reads or writes them: what converts to or from them, or moves them, is an extern kernel
+FLOAT8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e4m3fnuz, torch.float8_e5m2fnuz, torch.float8_e8m0fnu)
+
+
+def _install_float8_lowerings():
+    """Stock lowerings of conversions and copies, extern kernels where a tensor or the wanted type is an 8-bit float (the
+    result of ``b200_rmsnorm_quantised`` in a graph that does more with it than hand it to a product)."""
+    def is_float8(a):
+        dtype = a if isinstance(a, torch.dtype) else a.get_dtype() if isinstance(a, ir.IRNode) else None
+        return dtype in FLOAT8_DTYPES
+
+    for op in (prims.convert_element_type.default, aten.clone.default, aten.cat.default, aten.copy.default):
+        stock = lowerings.get(op)
+        if stock is None or getattr(stock, "_ixb_float8", False):
+            continue
+        extern = lowering.fallback_handler(op, add_to_fallback_set=False)
+
+        def guarded(*args, _stock=stock, _extern=extern, **kwargs):
+            return (_extern if any(map(is_float8, tree_leaves((args, kwargs)))) else _stock)(*args, **kwargs)
+
+        guarded._ixb_float8 = True
+        lowerings[op] = guarded
+
+
 def _register_b200_inductor_fallbacks():
     """Force the op families in ``FALLBACK_LIST`` to extern kernels.  Returns the overloads
     that were switched."""
     _install_scan_lowerings()
+    _install_float8_lowerings()
     targets = set()
     _init_set(FALLBACK_LIST + _special_function_ops(), targets)
     switched = []
