@@ -8,7 +8,9 @@
 //   norm_quantised_kernel          16-byte vectors of the row, where rows and pointers allow it
 //   norm_quantised_shifted_kernel  rows off a boundary: the vectors are those of memory, of which the row covers the first and
 //                                  the last in part
-//   norm_quantised_long_kernel     rows that no block holds, and operands that are off a boundary by different offsets
+//   norm_quantised_long_kernel     rows that no block holds, and operands that are off a boundary by different offsets: a view of
+//                                  x that starts off one, since q and h start on one (16384 x 4096 bf16 with residual 327 us,
+//                                  by vectors 72; 5003 x 1537 fp16 42, shifted 17)
 // Bound: memory, 2 (4 with residual) + 1 (3) bytes a value in 16 bits.
 #include <cuda_fp8.h>
 #include <atomic>

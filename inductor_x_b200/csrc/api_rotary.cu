@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_vector_kernel(const __grid
   }
 }
 
-// Heads that are no whole vectors, or off a boundary: a block a token, pair by pair.
+// Heads that are no whole vectors, or off a boundary: a block a token, pair by pair.  3 x 1369 tokens of 16 + 16 heads of 72 (36
+// pairs), fp16: 19.5 us, 1.94 TB/s (heads of 80 by vectors 11.4).
 template <class T> __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ float2 cs[kMaxPairs];
   const int b = blockIdx.x / p.S, s = blockIdx.x % p.S;

@@ -16,8 +16,9 @@
 // tile that holds it.
 //
 // Bound: as fa_fwd.cu, the chain scores -> softmax -> P -> product of a step and the drain between items.  8192 tokens of 32/8
-// heads, bf16, on one B200 at full clock: window 1024 137 us (fused_attention on nine unmasked steps 134), with 4 first tokens
-// 144 (as the last step of an item 150, all 128 keys of it 169), window 256 75, 2048 210; masks are 5 of it, stores 2.  Steps
+// heads, bf16, on one B200 at full clock: window 1024 132 - 137 us (fused_attention on nine unmasked steps 130 - 139), with 4 first
+// tokens 140 - 147, or 138 where K and V lie as in a cache (where they took 144 as the second step of an item, they took 150 as the
+// last one and 169 with all 128 keys of it), window 256 75 - 81, 2048 210 - 218; masks are 5 of it, stores 2.  Steps
 // from the window's beginning on 6 % more (rows that see nothing of the first tile rescale their accumulators);
 // the heads of one key head after the other instead of eight of them together 3 % more.
 #include <atomic>
