@@ -6,6 +6,8 @@
 // before the end, when the warps of a block and then the blocks of the cluster add up, row by row through distributed
 // shared memory: one launch, no scratch, the same bits every time.
 //
+// Probabilities are rounded to the operands' 16 bits, as in fa_window_fwd.cu; maxima, sums and accumulators have 32.
+//
 // Bound: memory.  A key costs 512 bytes and, per row, 512 multiplications, so that warp-wide 16 x 8 x 16 products are
 // enough.  They are taken with the keys (S^T = K Q^T) and the dimensions (O^T = V^T P^T) as their 16 rows and the queries as
 // their 8 columns, since hardly more than 8 queries share a key.  K and V come out of shared memory as whole 16-byte

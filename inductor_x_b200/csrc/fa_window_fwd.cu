@@ -15,6 +15,10 @@
 // looked at, but a probability of 0 times a NaN is one, so the producer clears the rows of V behind the length in the
 // tile that holds it.
 //
+// Probabilities are rounded to the operands' 16 bits, since P V is a product of 16-bit operands (32-bit ones take twice
+// the time and the memory); they are at most 2^8, relative to a maximum that may be stale by so much, and the sum that divides them is
+// of 32-bit values before that rounding.  The result is 1.3 to 1.4 times as far off as the same formula in 32 bits, rounded once.
+//
 // Bound: as fa_fwd.cu, the chain scores -> softmax -> P -> product of a step and the drain between items.  8192 tokens of 32/8
 // heads, bf16, on one B200 at full clock: window 1024 132 - 137 us (fused_attention on nine unmasked steps 130 - 139), with 4 first
 // tokens 140 - 147, or 138 where K and V lie as in a cache (where they took 144 as the second step of an item, they took 150 as the
