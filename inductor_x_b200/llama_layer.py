@@ -82,8 +82,9 @@ def window_attention_step(x, residual, w, positions, cache_k, cache_v, lengths, 
     """One token of each sequence: the residual is added and normalised to 8 bits, projected, turned and written to the
     cache at ``lengths`` (int32 [B], which it then advances), and attends to what its window leaves of the cache.
     x, residual [B, hidden], bf16 or fp16; w: dict with norm1 and, from :func:`quantise_rows`, wqkv, and wo; positions [axes, B, 1];
-    cache_k, cache_v [B, kv_heads, capacity, D], as :func:`ops.window_attention` takes them.  Returns the output projection and the new residual.  A sequence whose cache has
-    no room (nothing waits for the device to say so) keeps its cache and its length, and its projection is NaN."""
+    cache_k, cache_v [B, kv_heads, capacity, D], as :func:`ops.window_attention` takes them.  Returns the output projection and the
+    new residual.  A sequence whose cache has no room (nothing waits for the device to say so) keeps its cache and its length, and
+    its projection is NaN."""
     from . import ops
 
     # a call that is refused leaves the cache and the lengths as they are

@@ -452,8 +452,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     a padded batch or of what a cache holds: query ``i`` stands at position ``kv_lengths[b] - q_lengths[b] + i``, the
     last query at the last key.  A query that sees nothing, and any behind ``q_lengths[b]``, gets zeros and a
     log-sum-exp of ``-inf``.  What lies behind the lengths may be anything; values of ``v`` before them have to be finite (a NaN
-    or an infinity may reach queries that do not see its key, as a weight of 0 times it).  One to a few queries over a long cache are a decoding step: only the keys they see
-    are read.
+    or an infinity may reach queries that do not see its key, as a weight of 0 times it).  One to a few queries over a long
+    cache are a decoding step: only the keys they see are read.
 
     Returns ``out`` (contiguous ``[B, H, Sq, D]``) or ``(out, lse)``; ``check=True`` as in :func:`fused_attention`."""
     if not check:
@@ -483,8 +483,8 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               q_lengths: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
                               check: bool = False):
     """Gradients ``(dq, dk, dv)`` of :func:`window_attention` from its inputs, its output ``out``, its log-sum-exp
-    ``lse`` (``return_lse=True``) and the incoming gradient ``dout`` (any strides; the others' as there); ``dk`` and ``dv`` are sums over the query heads
-    that share a key head, and zero where no query sees the key.  Deterministic, no atomics."""
+    ``lse`` (``return_lse=True``) and the incoming gradient ``dout`` (any strides; the others' as there); ``dk`` and ``dv`` are
+    sums over the query heads that share a key head, and zero where no query sees the key.  Deterministic, no atomics."""
     if not check:
         done = _native("ixb_window_attention_bwd", _ixb_host.window_attention_backward(
             q, k, v, out, lse, dout, scale, window, sinks, q_lengths, kv_lengths))
